@@ -1,0 +1,106 @@
+// Element types, vector loads and activations shared by the layer kernels.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stddef.h>
+#include <stdint.h>
+
+#include "turbinator/training/hip_layers.h"
+
+namespace layer {
+
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+
+// Raw storage of B bytes, loaded and stored in one instruction.
+template <int B>
+struct Raw;
+template <>
+struct Raw<16> { typedef u32x4 type; };
+template <>
+struct Raw<8> { typedef u32x2 type; };
+template <>
+struct Raw<4> { typedef unsigned type; };
+template <>
+struct Raw<2> { typedef unsigned short type; };
+
+// B bytes of elements of type T as floats and back, rounded to nearest even.
+template <class T, int B>
+struct Vec {
+    static constexpr int n = B / (int)sizeof(T);
+    typedef typename Raw<B>::type raw;
+    typedef T elems __attribute__((ext_vector_type(n)));
+    typedef float floats __attribute__((ext_vector_type(n)));
+
+    static __device__ __forceinline__ void unpack(raw r, float (&v)[n]) {
+        const floats f = __builtin_convertvector(__builtin_bit_cast(elems, r), floats);
+#pragma unroll
+        for (int i = 0; i < n; ++i) v[i] = f[i];
+    }
+    static __device__ __forceinline__ raw pack(const float (&v)[n]) {
+        floats f;
+#pragma unroll
+        for (int i = 0; i < n; ++i) f[i] = v[i];
+        return __builtin_bit_cast(raw, __builtin_convertvector(f, elems));
+    }
+};
+
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr float kLog2eLow = 1.92596299112661887e-8f;  // log2(e) - kLog2e
+constexpr float kLn2 = 0.69314718055994530942f;
+
+// e^x.  v_exp_f32 is 2^x to 1 ulp; the rounding of x log2(e) alone would cost
+// |x| 2^-24, which a result rounded to 16 bits does not show.  With FINE the
+// product's remainder r is put back as the factor 1 + r ln 2, which keeps
+// about 2 ulp over the whole range.
+template <bool FINE>
+__device__ __forceinline__ float exp_of(float x) {
+    const float p = x * kLog2e;
+    const float e = __builtin_amdgcn_exp2f(p);
+    if constexpr (!FINE) return e;
+    const float r = fmaf(x, kLog2eLow, fmaf(x, kLog2e, -p));
+    // Past the range of floats e is 0 or inf and r may be NaN or huge.
+    return (p > -150.0f && p < 128.0f) ? fmaf(e, r * kLn2, e) : e;
+}
+
+// 1 / (1 + e^-z): v_rcp_f32 is within 1 ulp; FINE adds one Newton step, kept
+// off infinite denominators.
+template <bool FINE>
+__device__ __forceinline__ float sigmoid_of(float z) {
+    const float d = 1.0f + exp_of<FINE>(-z);
+    const float q = __builtin_amdgcn_rcpf(d);
+    if constexpr (!FINE) return q;
+    return d < 0x1p126f ? fmaf(fmaf(-d, q, 1.0f), q, q) : q;
+}
+
+template <bool FINE>
+__device__ __forceinline__ float act_of(float z, int act) {
+    if (act == TB_HIP_ACT_SILU) return z * sigmoid_of<FINE>(z);
+    if (act == TB_HIP_ACT_GELU) return 0.5f * z * (1.0f + erff(z * 0.70710678118654752440f));
+    return z;
+}
+
+// The derivative of act_of.
+template <bool FINE>
+__device__ __forceinline__ float act_slope(float z, int act) {
+    if (act == TB_HIP_ACT_SILU) {
+        const float s = sigmoid_of<FINE>(z);
+        return s * fmaf(z, 1.0f - s, 1.0f);
+    }
+    if (act == TB_HIP_ACT_GELU)
+        return 0.5f * (1.0f + erff(z * 0.70710678118654752440f)) +
+               z * (0.39894228040143267794f * exp_of<FINE>(-0.5f * z * z));
+    return 1.0f;
+}
+
+template <class T>
+constexpr bool kFine = sizeof(T) == 4;
+
+__host__ __device__ inline int type_size(int dtype) { return dtype == TB_HIP_F32 ? 4 : 2; }
+inline bool known_type(int dtype) {
+    return dtype == TB_HIP_F32 || dtype == TB_HIP_BF16 || dtype == TB_HIP_F16;
+}
+inline bool known_act(int act) { return act >= TB_HIP_ACT_NONE && act <= TB_HIP_ACT_GELU; }
+inline bool multiple_of(const void *p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+
+}  // namespace layer

@@ -1,0 +1,51 @@
+"""Python mirror of the layer entries (include/turbinator/training/hip_layers.h).
+
+Functions return 1 on success and 0 on refused arguments, exactly like the C
+entries they call; none allocates or waits.  Device arguments accept torch
+tensors on the GPU or raw device addresses; strides are bytes; `dtype` and
+`act` take the values of DTYPES and ACTS.
+"""
+from __future__ import annotations
+
+from .features import _dev, _stream
+from .native import hip_lib
+
+try:
+    import torch
+    DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+except ImportError:  # raw addresses need no torch
+    DTYPES = {}
+DTYPES.update({"f32": 0, "bf16": 1, "f16": 2})
+ACTS = {"none": 0, "silu": 1, "gelu": 2}
+
+
+def group_norm_workspace_bytes(images: int, pixels: int, channels: int, groups: int, dtype: int,
+                               backward: bool = False) -> int:
+    return hip_lib().tb_hip_group_norm_workspace_bytes(images, pixels, channels, groups, dtype,
+                                                       1 if backward else 0)
+
+
+def group_norm_device(x, image_stride: int, pixel_stride: int, gamma, beta, y, mean, rstd,
+                      workspace, images: int, pixels: int, channels: int, groups: int,
+                      eps: float, act: int, dtype: int, stream=None) -> int:
+    """tb_hip_group_norm_device."""
+    return hip_lib().tb_hip_group_norm_device(
+        _dev(x), image_stride, pixel_stride, _dev(gamma), _dev(beta), _dev(y), _dev(mean),
+        _dev(rstd), _dev(workspace), images, pixels, channels, groups, eps, act, dtype,
+        _stream(stream))
+
+
+def group_norm_backward_device(x, x_image_stride: int, x_pixel_stride: int, dy,
+                               dy_image_stride: int, dy_pixel_stride: int, gamma, beta, mean,
+                               rstd, dx, dgamma, dbeta, workspace, images: int, pixels: int,
+                               channels: int, groups: int, act: int, dtype: int,
+                               stream=None) -> int:
+    """tb_hip_group_norm_backward_device."""
+    return hip_lib().tb_hip_group_norm_backward_device(
+        _dev(x), x_image_stride, x_pixel_stride, _dev(dy), dy_image_stride, dy_pixel_stride,
+        _dev(gamma), _dev(beta), _dev(mean), _dev(rstd), _dev(dx), _dev(dgamma), _dev(dbeta),
+        _dev(workspace), images, pixels, channels, groups, act, dtype, _stream(stream))
+
+
+__all__ = ["DTYPES", "ACTS", "group_norm_workspace_bytes", "group_norm_device",
+           "group_norm_backward_device"]

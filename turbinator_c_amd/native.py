@@ -1,7 +1,7 @@
 """ctypes bindings of libturbinator_hip.so and libturbinator_synth.so.
 
 The product path is the C-ABI library; this module only declares its
-signatures (include/turbinator/training/cuda_features.h and hip_features.h)
+signatures (include/turbinator/training/cuda_features.h, hip_features.h and hip_layers.h)
 so Python callers, the tests and the benchmark call exactly what a C caller
 links.  Loading fails loudly when the library has not been built: there is no
 fallback implementation.
@@ -63,6 +63,14 @@ HIP_SIGNATURES = {
     "tb_hip_feature_pipeline_submit": (c_int, [c_void_p, c_int, c_size_t, c_int]),
     "tb_hip_feature_pipeline_submit_direct": (c_int, [c_void_p, c_int, c_size_t, c_int]),
     "tb_hip_feature_pipeline_wait": (c_void_p, [c_void_p, c_int]),
+    "tb_hip_group_norm_workspace_bytes":
+        (c_size_t, [c_size_t, c_size_t, c_int, c_int, c_int, c_int]),
+    "tb_hip_group_norm_device":
+        (c_int, [c_void_p, c_size_t, c_size_t] + [c_void_p] * 6 +
+         [c_size_t, c_size_t, c_int, c_int, c_float, c_int, c_int, c_void_p]),
+    "tb_hip_group_norm_backward_device":
+        (c_int, [c_void_p, c_size_t, c_size_t] * 2 + [c_void_p] * 8 +
+         [c_size_t, c_size_t, c_int, c_int, c_int, c_int, c_void_p]),
 }
 
 SYNTH_SIGNATURES = {
