@@ -3,7 +3,9 @@
  * (tb_hip_actor_inputs_device in hip_features.h), offered by the gfx950
  * backend (libturbinator_hip):
  *   - group norm with an activation over channels-last planes, forward and
- *     backward (the convolution stems).
+ *     backward (the convolution stems);
+ *   - routing of tokens to experts, forward and backward, and the order of
+ *     the choices by expert.
  * All pointers are device pointers.  All entries are asynchronous on `stream`
  * (a hipStream_t as void*, NULL = null stream), allocate nothing and return 1
  * iff the launches were accepted, 0 on invalid arguments (nothing is launched
@@ -20,13 +22,17 @@ extern "C" {
 #endif
 
 /* Element types of the `dtype` arguments, activations of the `act` arguments
- * (SiLU z / (1 + e^-z); GELU z Phi(z), Phi the normal distribution). */
+ * (SiLU z / (1 + e^-z); GELU z Phi(z), Phi the normal distribution) and
+ * scores of the `score` arguments. */
 enum { TB_HIP_F32 = 0, TB_HIP_BF16 = 1, TB_HIP_F16 = 2 };
 enum { TB_HIP_ACT_NONE = 0, TB_HIP_ACT_SILU = 1, TB_HIP_ACT_GELU = 2 };
+enum { TB_HIP_SCORE_SOFTMAX = 0, TB_HIP_SCORE_SIGMOID = 1 };
 
 enum {
     TB_HIP_NORM_MAX_GROUP = 1024,  /* channels of one group */
-    TB_HIP_NORM_MAX_CHANNELS = 65536
+    TB_HIP_NORM_MAX_CHANNELS = 65536,
+    TB_HIP_ROUTE_MAX_EXPERTS = 1024,
+    TB_HIP_ROUTE_MAX_K = 32
 };
 
 /* y = act((x - mean) rstd gamma + beta) over channels-last planes: `images`
@@ -71,6 +77,61 @@ int tb_hip_group_norm_backward_device(const void *x, size_t x_image_stride,
  * alignment; 0 for sizes they refuse. */
 size_t tb_hip_group_norm_workspace_bytes(size_t images, size_t pixels, int channels, int groups,
                                          int dtype, int backward);
+
+/* Routing: for each token (row of `logits`, row_stride bytes apart, n_experts
+ * values) the k experts of the highest keys, best first, equal keys in the
+ * order of their index, and their weights.
+ *   scores   s = softmax(logits) or sigmoid(logits), in 32 bits
+ *   keys     the logits, or s + bias with a bias ([n_experts] fp32, for
+ *            balance: it chooses and does not weigh)
+ *   groups   n_experts / groups consecutive experts each; only the
+ *            groups_kept best groups' experts are chosen from, a group's
+ *            standing being its best key, with a bias the sum of its two best
+ *   weights  scale s, with renormalise scale s / (sum of the token's chosen s)
+ *            (0 where that sum is 0)
+ * An expert whose logit or key is -inf is never chosen; where too few are
+ * left the remaining experts are -1 and their weights 0, and so is the whole
+ * row of a token whose `valid` byte (nullable, [tokens]) is 0, whose logits
+ * are not read.  NaN keys count as the highest and give NaN weights.
+ * experts [tokens, k] int32, weights [tokens, k] fp32.
+ * Returns 0 for NULL logits, experts or weights, tokens 0 or tokens * k above
+ * 0x7fffffff, n_experts outside 1..TB_HIP_ROUTE_MAX_EXPERTS, k outside
+ * 1..min(n_experts, TB_HIP_ROUTE_MAX_K), groups that do not divide n_experts,
+ * groups_kept outside 1..groups or of fewer than k experts together, an
+ * unknown score or dtype, logits or a stride off the element's size. */
+int tb_hip_route_device(const void *logits, size_t row_stride, const float *bias,
+                        const unsigned char *valid, int *experts, float *weights, size_t tokens,
+                        int n_experts, int k, int groups, int groups_kept, int score,
+                        int renormalise, float scale, int dtype, void *stream);
+
+/* The gradient dlogits (dense, the type of logits) of the weights for their
+ * gradient dweights [tokens, k], the choice held fixed.  experts as the
+ * forward pass chose them; those outside 0..n_experts-1 (-1) have no part,
+ * and a row of them alone has a zero gradient and is not read.  Same argument
+ * rules. */
+int tb_hip_route_backward_device(const void *logits, size_t row_stride, const int *experts,
+                                 const float *dweights, void *dlogits, size_t tokens,
+                                 int n_experts, int k, int score, int renormalise, float scale,
+                                 int dtype, void *stream);
+
+/* The tokens * k choices in the order of their experts, equal experts in the
+ * order of the choices (choice c = token c / k):
+ *   offsets [n_experts + 1]  expert x has rows offsets[x] .. offsets[x+1]-1
+ *   tokens_out [tokens * k]  the token of each row, -1 behind the last expert's
+ *   positions [tokens, k]    the row of each choice, -1 for a choice outside
+ *                            0..n_experts-1
+ *   row_weights [tokens * k] the weight of each row, 0 behind the last
+ *                            expert's; weights and row_weights may be NULL
+ *                            together
+ * workspace: tb_hip_expert_order_workspace_bytes(...) bytes, 16-byte aligned.
+ * Returns 0 for NULL pointers otherwise, tokens 0 or tokens * k above
+ * 0x7fffffff, n_experts outside 1..TB_HIP_ROUTE_MAX_EXPERTS or k outside
+ * 1..TB_HIP_ROUTE_MAX_K. */
+int tb_hip_expert_order_device(const int *experts, const float *weights, int *offsets,
+                               int *tokens_out, int *positions, float *row_weights,
+                               void *workspace, size_t tokens, int n_experts, int k,
+                               void *stream);
+size_t tb_hip_expert_order_workspace_bytes(size_t tokens, int n_experts, int k);
 
 #ifdef __cplusplus
 }

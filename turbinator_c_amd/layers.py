@@ -2,8 +2,8 @@
 
 Functions return 1 on success and 0 on refused arguments, exactly like the C
 entries they call; none allocates or waits.  Device arguments accept torch
-tensors on the GPU or raw device addresses; strides are bytes; `dtype` and
-`act` take the values of DTYPES and ACTS.
+tensors on the GPU or raw device addresses; strides are bytes; `dtype`, `act`
+and `score` take the values of DTYPES, ACTS and SCORES.
 """
 from __future__ import annotations
 
@@ -17,6 +17,7 @@ except ImportError:  # raw addresses need no torch
     DTYPES = {}
 DTYPES.update({"f32": 0, "bf16": 1, "f16": 2})
 ACTS = {"none": 0, "silu": 1, "gelu": 2}
+SCORES = {"softmax": 0, "sigmoid": 1}
 
 
 def group_norm_workspace_bytes(images: int, pixels: int, channels: int, groups: int, dtype: int,
@@ -47,5 +48,37 @@ def group_norm_backward_device(x, x_image_stride: int, x_pixel_stride: int, dy,
         _dev(workspace), images, pixels, channels, groups, act, dtype, _stream(stream))
 
 
-__all__ = ["DTYPES", "ACTS", "group_norm_workspace_bytes", "group_norm_device",
-           "group_norm_backward_device"]
+def route_device(logits, row_stride: int, bias, valid, experts, weights, tokens: int,
+                 n_experts: int, k: int, groups: int, groups_kept: int, score: int,
+                 renormalise: bool, scale: float, dtype: int, stream=None) -> int:
+    """tb_hip_route_device."""
+    return hip_lib().tb_hip_route_device(
+        _dev(logits), row_stride, _dev(bias), _dev(valid), _dev(experts), _dev(weights), tokens,
+        n_experts, k, groups, groups_kept, score, 1 if renormalise else 0, scale, dtype,
+        _stream(stream))
+
+
+def route_backward_device(logits, row_stride: int, experts, dweights, dlogits, tokens: int,
+                          n_experts: int, k: int, score: int, renormalise: bool, scale: float,
+                          dtype: int, stream=None) -> int:
+    """tb_hip_route_backward_device."""
+    return hip_lib().tb_hip_route_backward_device(
+        _dev(logits), row_stride, _dev(experts), _dev(dweights), _dev(dlogits), tokens,
+        n_experts, k, score, 1 if renormalise else 0, scale, dtype, _stream(stream))
+
+
+def expert_order_workspace_bytes(tokens: int, n_experts: int, k: int) -> int:
+    return hip_lib().tb_hip_expert_order_workspace_bytes(tokens, n_experts, k)
+
+
+def expert_order_device(experts, weights, offsets, tokens_out, positions, row_weights, workspace,
+                        tokens: int, n_experts: int, k: int, stream=None) -> int:
+    """tb_hip_expert_order_device."""
+    return hip_lib().tb_hip_expert_order_device(
+        _dev(experts), _dev(weights), _dev(offsets), _dev(tokens_out), _dev(positions),
+        _dev(row_weights), _dev(workspace), tokens, n_experts, k, _stream(stream))
+
+
+__all__ = ["DTYPES", "ACTS", "SCORES", "group_norm_workspace_bytes", "group_norm_device",
+           "group_norm_backward_device", "route_device", "route_backward_device",
+           "expert_order_workspace_bytes", "expert_order_device"]

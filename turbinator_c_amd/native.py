@@ -71,6 +71,15 @@ HIP_SIGNATURES = {
     "tb_hip_group_norm_backward_device":
         (c_int, [c_void_p, c_size_t, c_size_t] * 2 + [c_void_p] * 8 +
          [c_size_t, c_size_t, c_int, c_int, c_int, c_int, c_void_p]),
+    "tb_hip_route_device":
+        (c_int, [c_void_p, c_size_t] + [c_void_p] * 4 +
+         [c_size_t] + [c_int] * 6 + [c_float, c_int, c_void_p]),
+    "tb_hip_route_backward_device":
+        (c_int, [c_void_p, c_size_t] + [c_void_p] * 3 +
+         [c_size_t] + [c_int] * 4 + [c_float, c_int, c_void_p]),
+    "tb_hip_expert_order_workspace_bytes": (c_size_t, [c_size_t, c_int, c_int]),
+    "tb_hip_expert_order_device":
+        (c_int, [c_void_p] * 7 + [c_size_t, c_int, c_int, c_void_p]),
 }
 
 SYNTH_SIGNATURES = {
