@@ -5,7 +5,9 @@
  *   - group norm with an activation over channels-last planes, forward and
  *     backward (the convolution stems);
  *   - routing of tokens to experts, forward and backward, and the order of
- *     the choices by expert.
+ *     the choices by expert;
+ *   - microscaled 4-bit floating point: quantisation, its values, and
+ *     products on the scaled matrix instructions, dense or per expert.
  * All pointers are device pointers.  All entries are asynchronous on `stream`
  * (a hipStream_t as void*, NULL = null stream), allocate nothing and return 1
  * iff the launches were accepted, 0 on invalid arguments (nothing is launched
@@ -32,7 +34,8 @@ enum {
     TB_HIP_NORM_MAX_GROUP = 1024,  /* channels of one group */
     TB_HIP_NORM_MAX_CHANNELS = 65536,
     TB_HIP_ROUTE_MAX_EXPERTS = 1024,
-    TB_HIP_ROUTE_MAX_K = 32
+    TB_HIP_ROUTE_MAX_K = 32,
+    TB_HIP_MX4_BLOCK = 32          /* values that share a scale */
 };
 
 /* y = act((x - mean) rstd gamma + beta) over channels-last planes: `images`
@@ -132,6 +135,47 @@ int tb_hip_expert_order_device(const int *experts, const float *weights, int *of
                                void *workspace, size_t tokens, int n_experts, int k,
                                void *stream);
 size_t tb_hip_expert_order_workspace_bytes(size_t tokens, int n_experts, int k);
+
+/* Microscaled 4-bit floating point (the OCP MX format MXFP4): 32 consecutive
+ * values of a row share a scale 2^(s - 127), s one byte, and are held as sign,
+ * two exponent bits and one mantissa bit (0, 0.5, 1, 1.5, 2, 3, 4, 6).  A row
+ * of k values is padded with zeros to kp = tb_hip_mx4_padded(k), whole 128s:
+ * codes [rows, kp / 2] bytes, the even value in the low half; scales
+ * [rows, kp / 32] bytes.  codes must be 16-byte, scales 4-byte aligned.
+ *
+ * Quantisation: s - 127 = floor(log2(largest magnitude)) - 2, at least -127;
+ * values rounded to nearest, ties to even, magnitudes above 6 to 6.  A block
+ * that holds an Inf or a NaN has s = 255 (NaN) and zero codes. */
+size_t tb_hip_mx4_padded(size_t k);
+int tb_hip_mx4_quantise_device(const void *x, size_t row_stride, void *codes, void *scales,
+                               size_t rows, size_t k, int dtype, void *stream);
+
+/* The values [rows, k] (dense) that codes and scales stand for, rounded to
+ * the type (only f16 can round or overflow).
+ * Both return 0 for NULL pointers, rows or k 0 or above 0x7fffffff, an
+ * unknown dtype or misaligned pointers or stride. */
+int tb_hip_mx4_values_device(const void *codes, const void *scales, void *values, size_t rows,
+                             size_t k, int dtype, void *stream);
+
+/* out[r] = act(A[a(r)] W[x(r)]^T + bias[x(r)]) row_scale[r]: products of
+ * quantised rows, summed in 32 bits and rounded once.  A: a_rows rows of k.
+ * W: experts * n rows of k, bias [experts, n] fp32 (nullable), row_scale [m]
+ * fp32 (nullable).
+ *   a(r) = rows[r], or r with rows NULL (then m = a_rows)
+ *   x(r) = the expert with offsets[x] <= r < offsets[x+1]; experts = 1 and
+ *          offsets NULL for one dense product
+ * Rows that belong to no expert, or whose rows[r] is outside 0..a_rows-1,
+ * come out as 0.  offsets must not decrease; entries are taken as at least 0
+ * and at most m.  out [m, n] is dense.
+ * Returns 0 for other NULL pointers, m, n, k or a_rows 0 or above 0x7fffffff,
+ * experts outside 1..TB_HIP_ROUTE_MAX_EXPERTS or above 1 without offsets,
+ * experts * n above 0x7fffffff, rows NULL with m other than a_rows, an
+ * unknown act or dtype, or misaligned pointers. */
+int tb_hip_mx4_product_device(const void *a_codes, const void *a_scales, size_t a_rows,
+                              const int *rows, const void *w_codes, const void *w_scales,
+                              const int *offsets, const float *bias, const float *row_scale,
+                              void *out, size_t m, size_t n, size_t k, int experts, int act,
+                              int dtype, void *stream);
 
 #ifdef __cplusplus
 }

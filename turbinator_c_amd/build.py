@@ -37,7 +37,8 @@ HIP_FLAGS = [
 C_FLAGS = ["-O2", "-std=c11", "-fPIC", "-Wall", "-Wextra", "-D__HIP_PLATFORM_AMD__",
            f"-I{ROCM / 'include'}", f"-I{INCLUDE}"]
 
-HIP_SOURCES = ["features.hip", "onboard.hip", "sac_actor.hip", "group_norm.hip", "route.hip"]
+HIP_SOURCES = ["features.hip", "onboard.hip", "sac_actor.hip", "group_norm.hip", "route.hip",
+               "mx4.hip"]
 HOST_C_SOURCES = ["feature_batch.c", "feature_pipeline.c", "sac_host.c"]
 
 LIB_HIP = PKG / "libturbinator_hip.so"

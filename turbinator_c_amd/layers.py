@@ -18,6 +18,7 @@ except ImportError:  # raw addresses need no torch
 DTYPES.update({"f32": 0, "bf16": 1, "f16": 2})
 ACTS = {"none": 0, "silu": 1, "gelu": 2}
 SCORES = {"softmax": 0, "sigmoid": 1}
+MX4_BLOCK = 32
 
 
 def group_norm_workspace_bytes(images: int, pixels: int, channels: int, groups: int, dtype: int,
@@ -79,6 +80,34 @@ def expert_order_device(experts, weights, offsets, tokens_out, positions, row_we
         _dev(row_weights), _dev(workspace), tokens, n_experts, k, _stream(stream))
 
 
-__all__ = ["DTYPES", "ACTS", "SCORES", "group_norm_workspace_bytes", "group_norm_device",
-           "group_norm_backward_device", "route_device", "route_backward_device",
-           "expert_order_workspace_bytes", "expert_order_device"]
+def mx4_padded(k: int) -> int:
+    return hip_lib().tb_hip_mx4_padded(k)
+
+
+def mx4_quantise_device(x, row_stride: int, codes, scales, rows: int, k: int, dtype: int,
+                        stream=None) -> int:
+    """tb_hip_mx4_quantise_device."""
+    return hip_lib().tb_hip_mx4_quantise_device(_dev(x), row_stride, _dev(codes), _dev(scales),
+                                                rows, k, dtype, _stream(stream))
+
+
+def mx4_values_device(codes, scales, values, rows: int, k: int, dtype: int, stream=None) -> int:
+    """tb_hip_mx4_values_device."""
+    return hip_lib().tb_hip_mx4_values_device(_dev(codes), _dev(scales), _dev(values), rows, k,
+                                              dtype, _stream(stream))
+
+
+def mx4_product_device(a_codes, a_scales, a_rows: int, rows, w_codes, w_scales, offsets, bias,
+                       row_scale, out, m: int, n: int, k: int, experts: int, act: int,
+                       dtype: int, stream=None) -> int:
+    """tb_hip_mx4_product_device."""
+    return hip_lib().tb_hip_mx4_product_device(
+        _dev(a_codes), _dev(a_scales), a_rows, _dev(rows), _dev(w_codes), _dev(w_scales),
+        _dev(offsets), _dev(bias), _dev(row_scale), _dev(out), m, n, k, experts, act, dtype,
+        _stream(stream))
+
+
+__all__ = ["DTYPES", "ACTS", "SCORES", "MX4_BLOCK", "group_norm_workspace_bytes",
+           "group_norm_device", "group_norm_backward_device", "route_device",
+           "route_backward_device", "expert_order_workspace_bytes", "expert_order_device",
+           "mx4_padded", "mx4_quantise_device", "mx4_values_device", "mx4_product_device"]

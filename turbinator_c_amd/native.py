@@ -80,6 +80,14 @@ HIP_SIGNATURES = {
     "tb_hip_expert_order_workspace_bytes": (c_size_t, [c_size_t, c_int, c_int]),
     "tb_hip_expert_order_device":
         (c_int, [c_void_p] * 7 + [c_size_t, c_int, c_int, c_void_p]),
+    "tb_hip_mx4_padded": (c_size_t, [c_size_t]),
+    "tb_hip_mx4_quantise_device":
+        (c_int, [c_void_p, c_size_t, c_void_p, c_void_p, c_size_t, c_size_t, c_int, c_void_p]),
+    "tb_hip_mx4_values_device":
+        (c_int, [c_void_p] * 3 + [c_size_t, c_size_t, c_int, c_void_p]),
+    "tb_hip_mx4_product_device":
+        (c_int, [c_void_p, c_void_p, c_size_t] + [c_void_p] * 7 +
+         [c_size_t, c_size_t, c_size_t, c_int, c_int, c_int, c_void_p]),
 }
 
 SYNTH_SIGNATURES = {
