@@ -311,6 +311,15 @@ def test_gradient(torch_cuda, n, k, score, renorm, dtype):
 
 
 @pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+def test_a_single_renormalised_choice_has_no_gradient(torch_cuda, score):
+    x = logits_of(5, 40, 24, torch.float32)
+    experts, weights = route(x, 1, score, True)
+    assert (weights == 1).all()
+    dw = torch.randn(experts.shape, generator=torch.Generator().manual_seed(3)).cuda()
+    assert (backward(x, experts, dw, score, True, 1.0) == 0).all()
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
 @pytest.mark.parametrize("renorm", [True, False])
 def test_gradient_of_partial_and_empty_rows(torch_cuda, score, renorm):
     x = logits_of(5, 40, 24, torch.float32)

@@ -246,7 +246,8 @@ __global__ __launch_bounds__(kThreads) void route_backward_kernel(RouteArgs a) {
         if (live)
             for (int i = 0; i < a.k; ++i) used += (unsigned)at[i] < (unsigned)a.n;
         if (a.renorm) {
-            // w' of the chosen from their logits alone; sum g w' first.
+            // w' of the chosen from their logits alone, as quotients: a single
+            // choice has w' = 1 and no gradient, exactly.
             float most = -__builtin_inff(), total = 0.0f, dot = 0.0f;
             if (used) {
                 if (soft)
@@ -256,24 +257,29 @@ __global__ __launch_bounds__(kThreads) void route_backward_kernel(RouteArgs a) {
                 for (int i = 0; i < a.k; ++i)
                     if ((unsigned)at[i] < (unsigned)a.n) {
                         const float x = element<T>(row, at[i]);
-                        const float s = soft ? exp_of<true>(x - most) : sigmoid_of<true>(x);
-                        total += s;
-                        dot += s * (a.scale * dw[i]);
+                        total += soft ? exp_of<true>(x - most) : sigmoid_of<true>(x);
                     }
+                // A sum of 0 gave weights of 0.
+                if (total == 0.0f) used = 0;
             }
-            const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
-            dot *= inverse;
-            if (used)
+            if (used) {
+                for (int i = 0; i < a.k; ++i)
+                    if ((unsigned)at[i] < (unsigned)a.n) {
+                        const float x = element<T>(row, at[i]);
+                        const float s = soft ? exp_of<true>(x - most) : sigmoid_of<true>(x);
+                        dot += s / total * (a.scale * dw[i]);
+                    }
                 for (int i = 0; i < a.k; ++i)
                     if (at[i] >= e0 && at[i] < e0 + Q && at[i] < a.n) {
                         const float x = element<T>(row, at[i]);
                         const float s = soft ? exp_of<true>(x - most) : sigmoid_of<true>(x);
                         // 1 - s as the sigmoid of -x, without cancelling.
                         const float rest = soft ? 1.0f : sigmoid_of<true>(-x);
-                        const float v = s * inverse * rest * (a.scale * dw[i] - dot);
+                        const float v = s / total * rest * (a.scale * dw[i] - dot);
 #pragma unroll
                         for (int j = 0; j < Q; ++j) d[j] += at[i] == e0 + j ? v : 0.0f;
                     }
+            }
         } else {
             if (used)
                 for (int i = 0; i < a.k; ++i)
