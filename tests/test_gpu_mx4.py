@@ -225,6 +225,10 @@ SIZES = [(1, 1, 1), (1, 16, 128), (2, 17, 33), (10, 64, 512), (15, 100, 129), (1
          (17, 256, 1000), (33, 130, 640), (64, 64, 4096), (65, 1000, 100), (100, 300, 300),
          (129, 127, 1500), (256, 512, 256), (300, 260, 128), (513, 511, 384), (1000, 1024, 1024),
          (10, 4096, 4096), (320, 2048, 2048), (2050, 96, 70)]
+# Every shape of the product: few rows with one, two and four row tiles, staged
+# tiles of 128 and of 256; widths with one to eight steps of 128; ragged ends.
+SIZES += [(m, n, k) for m, n in ((33, 1500), (60, 2100), (200, 9000), (700, 500), (1300, 1111),
+                                 (4200, 2200)) for k in (100, 250, 300, 500, 512, 700, 900, 1024)]
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=str)

@@ -10,6 +10,7 @@
 //          v_mfma_scale_f32_16x16x128_f8f6f4: lane l holds row l % 16, values
 //          32 (l / 16) .. + 31 of a step of 128, one scale block, in 16 bytes
 #include "layer_math.h"
+#include "xcd_order.h"
 
 namespace {
 
@@ -196,16 +197,17 @@ __device__ __forceinline__ bool find_rows(const ProductArgs &a, size_t tile, int
         const unsigned long long reach = __ballot(tile < sum);
         if (reach) {
             const int at = __ffsll(reach) - 1;
-            const unsigned before = __shfl(sum - tiles, at);
+            // Counts below 2^31, the same for the whole wave.
+            const size_t before = __builtin_amdgcn_readlane(sum - tiles, at);
+            lo = (unsigned)__builtin_amdgcn_readlane((int)lo, at);
+            hi = (unsigned)__builtin_amdgcn_readlane((int)hi, at);
             const int expert = base + at - 1;
-            lo = __shfl((unsigned long long)lo, at);
-            hi = __shfl((unsigned long long)hi, at);
             t.expert = expert < 0 ? a.experts : expert;
             t.r0 = lo + (tile - before) * height;
             t.r1 = t.r0 + height < hi ? t.r0 + height : hi;
             return true;
         }
-        tile -= __shfl(sum, 63);
+        tile -= __builtin_amdgcn_readlane(sum, 63);
     }
     return false;
 }
@@ -240,62 +242,454 @@ __device__ __forceinline__ void store4(const ProductArgs &a, int expert, bool re
     }
 }
 
-// Tiles of 64 columns and 64 rows, 32 by 32 a wave, operands straight from
-// memory in the instruction's layout.  The weights are the first operand, so
-// a lane ends with four consecutive columns of one row.
-constexpr int kTile = 64;
+// Few rows: tiles of 16 columns and 16 MT rows, operands straight from memory
+// in the instruction's layout, k split over the workgroup's waves in pairs of
+// steps (128 bytes of a row) and joined in LDS.  The weights are the first
+// operand, so a lane ends with four consecutive columns of one row.
+constexpr int kFewWaves = 8;
 
-template <class T>
-__global__ __launch_bounds__(256) void product_kernel(ProductArgs a) {
-    const int t = threadIdx.x, wave = t >> 6, lane = t & 63, low = lane & 15, part = lane >> 4;
-    const size_t columns = (a.n + kTile - 1) / kTile;
-    const size_t tile = blockIdx.x / columns;
+template <class T, int MT>
+__global__ __launch_bounds__(64 * kFewWaves) void few_kernel(ProductArgs a) {
+    __shared__ f32x4 sums[kFewWaves][MT][64];
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const int low = lane & 15, part = lane >> 4;
+    const unsigned columns = (unsigned)((a.n + 15) / 16), tile = blockIdx.x / columns;
     RowTile rt;
-    if (!find_rows(a, tile, kTile, rt)) return;
-    const size_t n0 = (blockIdx.x - tile * columns) * kTile + (wave & 1) * 32;
-    const size_t m0 = rt.r0 + (wave >> 1) * 32;
-    const size_t codes = a.kp / 2, scales = a.kp / kBlock;
-    f32x4 acc[2][2] = {};
-    const unsigned char *wc[2], *ws[2], *xc[2], *xs[2];
-    bool real[2];
+    if (!find_rows(a, tile, 16 * MT, rt)) return;
+    const size_t n0 = (size_t)(blockIdx.x - tile * columns) * 16;
+    const bool some = rt.expert < a.experts;
+    const size_t code_row = a.kp / 2, scale_row = a.kp / kBlock;
+    const size_t wr = (n0 + low < a.n ? n0 + low : a.n - 1) + (some ? rt.expert * a.n : 0);
+    const unsigned char *wc = a.w_codes + wr * code_row + part * 16;
+    const unsigned char *ws = a.w_scales + wr * scale_row + part;
+    const unsigned char *xc[MT], *xs[MT];
+    unsigned real = 0;  // a bit for each row tile
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        size_t r = n0 + i * 16 + low;
-        r = (r < a.n ? r : a.n - 1) + (rt.expert < a.experts ? rt.expert * a.n : 0);
-        wc[i] = a.w_codes + r * codes + part * 16;
-        ws[i] = a.w_scales + r * scales + part;
-        size_t m = m0 + i * 16 + low;
+    for (int j = 0; j < MT; ++j) {
+        size_t m = rt.r0 + j * 16 + low;
         m = m < rt.r1 ? m : rt.r1 - 1;
         const long long row = a.rows ? a.rows[m] : (long long)m;
-        real[i] = rt.expert < a.experts && row >= 0 && (size_t)row < a.a_rows;
-        xc[i] = a.a_codes + (real[i] ? row : 0) * codes + part * 16;
-        xs[i] = a.a_scales + (real[i] ? row : 0) * scales + part;
+        const bool there = row >= 0 && (size_t)row < a.a_rows;
+        real |= (some && there ? 1u : 0u) << j;
+        xc[j] = a.a_codes + (there ? row : 0) * code_row + part * 16;
+        xs[j] = a.a_scales + (there ? row : 0) * scale_row + part;
     }
-    if (rt.expert < a.experts)
-        for (size_t k = 0; k < a.kp; k += kPad) {
-            i32x4 w[2], x[2];
-            int sw[2], sx[2];
+    f32x4 acc[MT];
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                w[i] = *reinterpret_cast<const i32x4 *>(wc[i] + k / 2);
-                x[i] = *reinterpret_cast<const i32x4 *>(xc[i] + k / 2);
-                sw[i] = ws[i][k / kBlock];
-                sx[i] = xs[i][k / kBlock];
+    for (int j = 0; j < MT; ++j) acc[j] = (f32x4){0, 0, 0, 0};
+    const size_t steps = some ? a.kp / kPad : 0;
+    for (size_t s = 2 * wave; s < steps; s += 2 * kFewWaves) {
+        // A step behind the last is the last again, times nothing.
+        const size_t next = s + 1 < steps ? s + 1 : s;
+        const i32x4 w0 = *reinterpret_cast<const i32x4 *>(wc + s * 64);
+        const i32x4 w1 = *reinterpret_cast<const i32x4 *>(wc + next * 64);
+        const int sw0 = ws[s * 4], sw1 = ws[next * 4];
+        i32x4 x0[MT], x1[MT];
+        int sx0[MT], sx1[MT];
+#pragma unroll
+        for (int j = 0; j < MT; ++j) {
+            x0[j] = *reinterpret_cast<const i32x4 *>(xc[j] + s * 64);
+            x1[j] = *reinterpret_cast<const i32x4 *>(xc[j] + next * 64);
+            sx0[j] = xs[j][s * 4];
+            sx1[j] = xs[j][next * 4];
+        }
+#pragma unroll
+        for (int j = 0; j < MT; ++j) acc[j] = step16(w0, sw0, x0[j], sx0[j], acc[j]);
+        if (next > s)
+#pragma unroll
+            for (int j = 0; j < MT; ++j) acc[j] = step16(w1, sw1, x1[j], sx1[j], acc[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < MT; ++j) sums[wave][j][lane] = acc[j];
+    __syncthreads();
+    for (int j = wave; j < MT; j += kFewWaves) {
+        f32x4 sum = sums[0][j][lane];
+        for (int w = 1; w < kFewWaves; ++w) sum += sums[w][j][lane];
+        const size_t r = rt.r0 + j * 16 + low, c = n0 + part * 4;
+        if (r < rt.r1 && c < a.n) store4<T>(a, rt.expert, real >> j & 1, r, c, sum);
+    }
+}
+
+// Large products: tiles of BM rows and BN columns, staged through LDS in
+// slices of two steps (256 values, 128 bytes a row), two slices in turn.
+//
+// Codes come by loads that write LDS themselves: a wave's load fills 1 KB,
+// eight rows, in lane order.  16-byte piece c of row r lies at slot c ^ (r & 7)
+// of its row, so that the rows of an operand read, 128 bytes apart, fall on
+// all banks.  Scales come through registers, the eight of a row at once (a
+// request of the L2 costs the same for four bytes as for a line), and are
+// turned while they are stored: lane l's word holds the scales of its part of
+// four row tiles, which the instruction picks by number.
+//
+// Turn s: read step 1 of slice s while multiplying step 0; wait for the loads
+// of slice s + 1; barrier: all waves have them, and have read slice s; load
+// slice s + 2 over it, and read step 0 of slice s + 1 while multiplying step 1.
+constexpr int kSlice = 2 * kPad, kSliceBytes = kSlice / 2;
+
+typedef const __attribute__((address_space(1))) void *GlobalPtr;
+typedef __attribute__((address_space(3))) void *LdsPtr;
+typedef __attribute__((address_space(3))) unsigned char *LdsBytes;
+
+__device__ __forceinline__ void load_to_lds(const void *from, void *to) {
+    __builtin_amdgcn_global_load_lds((GlobalPtr)from, (LdsPtr)to, 16, 0, 0);
+}
+
+// Waits for the wave's loads and LDS accesses, then for the other waves.
+__device__ __forceinline__ void arrive() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0)
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("" ::: "memory");
+}
+
+__device__ __forceinline__ f32x4 step_of(int sel, i32x4 w, int ws, i32x4 x, int xs, f32x4 c) {
+    const i32x8 A = {w[0], w[1], w[2], w[3], 0, 0, 0, 0}, B = {x[0], x[1], x[2], x[3], 0, 0, 0, 0};
+#define TB_STEP(i, j)                                                                       \
+    case 4 * i + j:                                                                         \
+        return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(A, B, c, 4, 4, i, ws, j, xs);
+    switch (sel) {
+        TB_STEP(0, 0) TB_STEP(0, 1) TB_STEP(0, 2) TB_STEP(0, 3)
+        TB_STEP(1, 0) TB_STEP(1, 1) TB_STEP(1, 2) TB_STEP(1, 3)
+        TB_STEP(2, 0) TB_STEP(2, 1) TB_STEP(2, 2) TB_STEP(2, 3)
+        TB_STEP(3, 0) TB_STEP(3, 1) TB_STEP(3, 2)
+        default:
+            return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(A, B, c, 4, 4, 3, ws, 3, xs);
+    }
+#undef TB_STEP
+}
+
+// The most row tiles, halving from `all`, whose `bytes` each fit into `room`.
+constexpr int pass_tiles(int all, int bytes, int room) {
+    return all * bytes <= room ? all : pass_tiles(all / 2, bytes, room);
+}
+
+// The operands of one step of a wave: MT row tiles and NT column tiles.
+template <int MT, int NT>
+struct Operands {
+    i32x4 x[MT], w[NT];
+    int xs[MT / 4], ws[NT / 4];
+};
+
+// Lane 16 j + r holds the four scale bytes of row 16 j + r: out, lane 16 p + r
+// holds byte p of the rows r, 16 + r, 32 + r and 48 + r.  Two exchanges between
+// lanes 32 and 16 apart, each followed by a choice of bytes.
+__device__ __forceinline__ int turned(unsigned v, int p) {
+    const auto far = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    v = __builtin_amdgcn_perm(far[1], far[0], p & 2 ? 0x07060302 : 0x05040100);
+    const auto near = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    return (int)__builtin_amdgcn_perm(near[1], near[0], p & 1 ? 0x07030501 : 0x06020400);
+}
+
+// `codes` and `scales` at the lane's place of step 0 or 1.
+template <int MT, int NT>
+__device__ __forceinline__ void read_step(const unsigned char *__restrict codes,
+                                          const int *__restrict scales, int row_x, int row_w,
+                                          Operands<MT, NT> &__restrict o) {
+#pragma unroll
+    for (int j = 0; j < MT / 4; ++j) o.xs[j] = scales[row_x * 2 + j * 128];
+#pragma unroll
+    for (int i = 0; i < NT / 4; ++i) o.ws[i] = scales[row_w * 2 + i * 128];
+#pragma unroll
+    for (int j = 0; j < MT; ++j)
+        o.x[j] = *reinterpret_cast<const i32x4 *>(codes + row_x * kSliceBytes +
+                                                  j * 16 * kSliceBytes);
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+        o.w[i] = *reinterpret_cast<const i32x4 *>(codes + row_w * kSliceBytes +
+                                                  i * 16 * kSliceBytes);
+}
+
+template <int MT, int NT>
+__device__ __forceinline__ void multiply(const Operands<MT, NT> &o, f32x4 (&acc)[NT][MT]) {
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+        for (int j = 0; j < MT; ++j)
+            acc[i][j] = step_of(4 * (i % 4) + j % 4, o.w[i], o.ws[i / 4], o.x[j], o.xs[j / 4],
+                                acc[i][j]);
+}
+
+// Eight consecutive columns n0 .. of row r.
+template <class T>
+__device__ __forceinline__ void store8(const ProductArgs &a, size_t r, size_t n0,
+                                       const float (&v)[8]) {
+    T *out = reinterpret_cast<T *>(a.out) + r * a.n + n0;
+    if (a.vector && n0 + 8 <= a.n) {
+        typedef Vec<T, 16> X;
+#pragma unroll
+        for (int p = 0; p < 8 / X::n; ++p) {
+            float part[X::n];
+#pragma unroll
+            for (int i = 0; i < X::n; ++i) part[i] = v[p * X::n + i];
+            *reinterpret_cast<typename X::raw *>(out + p * X::n) = X::pack(part);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (n0 + i < a.n) out[i] = (T)v[i];
+    }
+}
+
+template <class T, int ACT, int WM, int WN, int MT, int NT>
+__global__ __launch_bounds__(64 * WM * WN) void tile_kernel(ProductArgs a) {
+    constexpr int BM = 16 * MT * WM, BN = 16 * NT * WN, kWaves = WM * WN, kThreads = 64 * kWaves;
+    constexpr int kRows = BM + BN, kLoads = kRows / 8 / kWaves;  // 1 KB a load of a wave
+    constexpr int kReads = MT + NT + 2;  // of a step
+    static_assert(kRows == kThreads && BM % (kLoads * 8) == 0);
+    constexpr int kGroup = 8;  // column tiles that neighbours in time share
+    // Two arrays each, chosen at compile time: the compiler knows that a read
+    // of one need not wait for the loads into the other.
+    __shared__ __attribute__((aligned(1024))) unsigned char codes0[kRows * kSliceBytes];
+    __shared__ __attribute__((aligned(1024))) unsigned char codes1[kRows * kSliceBytes];
+    __shared__ __attribute__((aligned(4096))) int scales0[kRows * 2], scales1[kRows * 2];  // [group of 64 rows][step][lane]
+    // Byte offset of each row's codes, by the loading wave, lane / 8 and load.
+    __shared__ __attribute__((aligned(16))) unsigned row_code[kRows];
+    __shared__ float scale_of_row[BM];
+    __shared__ unsigned char real_row[BM];
+
+    const int t = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t >> 6), lane = t & 63;
+    const int low = lane & 15, part = lane >> 4;
+    const int wm = wave % WM, wn = wave / WM;
+    const unsigned columns = (unsigned)((a.n + BN - 1) / BN), heights = gridDim.x / columns;
+    const unsigned at = (unsigned)xcd_contiguous(blockIdx.x, gridDim.x);
+    const unsigned band = at / (kGroup * heights), rest = at - band * kGroup * heights;
+    const unsigned wide = columns - band * kGroup < kGroup ? columns - band * kGroup : kGroup;
+    RowTile rt;
+    if (!find_rows(a, rest / wide, BM, rt)) return;
+    const size_t n0 = (size_t)(band * kGroup + rest % wide) * BN, m0 = rt.r0;
+    const int height = (int)(rt.r1 - rt.r0);
+    const bool none = rt.expert >= a.experts;
+    const size_t code_row = a.kp / 2, scale_row = a.kp / kBlock;
+    const size_t w_first = none ? 0 : (size_t)rt.expert * a.n;
+
+    if (none) {
+        const float zeros[8] = {};
+        const size_t c = n0 + t % (BN / 8) * 8;
+        for (int r = t / (BN / 8); r < height; r += kThreads * 8 / BN)
+            if (c < a.n) store8<T>(a, m0 + r, c, zeros);
+        return;
+    }
+    // The matrix row behind each row of the tile, the output's rows first,
+    // counted from the tile's first (from the matrix's where they are
+    // gathered; row 0 is read for one that is not there); rows past the tile's
+    // end stand in for the last one and are not stored.
+    int row;
+    if (t >= BM) {
+        row = n0 + (t - BM) < a.n ? t - BM : (int)(a.n - 1 - n0);
+    } else {
+        const int in = t < height ? t : height - 1;
+        row = a.rows ? a.rows[m0 + in] : in;
+        const bool real = !a.rows || (row >= 0 && (size_t)row < a.a_rows);
+        row = real ? row : 0;
+        real_row[t] = real;
+        scale_of_row[t] = a.row_scale ? a.row_scale[m0 + in] : 1.0f;
+    }
+    row_code[(t / (8 * kLoads) * 8 + t % 8) * kLoads + t / 8 % kLoads] = (unsigned)(row * code_row);
+    __syncthreads();
+
+    f32x4 acc[NT][MT];
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+        for (int j = 0; j < MT; ++j) acc[i][j] = (f32x4){0, 0, 0, 0};
+
+    // Codes: a base of the wave's side, 32 bits to the row, and a column that
+    // stays within it (the second step of a last slice may lie past its end:
+    // what is read for it is not used).
+    const int row0 = wave * kLoads * 8;
+    const bool w_side = row0 >= BM;
+    const size_t first = w_side ? w_first + n0 : a.rows ? 0 : m0;
+    const unsigned char *base = (w_side ? a.w_codes : a.a_codes) + first * code_row;
+    unsigned from[kLoads];
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) from[i] = row_code[(t >> 3) * kLoads + i];
+    const unsigned column = ((lane & 7) ^ (lane >> 3)) * 16, code_end = (unsigned)code_row - 16;
+    auto load = [&](unsigned slice, unsigned char *codes) {
+        unsigned at = slice * kSliceBytes + column;
+        at = at < code_end ? at : code_end;
+        unsigned char *to = codes + row0 * kSliceBytes;
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) load_to_lds(base + (from[i] + at), to + i * 1024);
+    };
+    // Scales: thread t has row t, on the same side as its wave's chunks.
+    const unsigned char *sbase = (w_side ? a.w_scales : a.a_scales) + first * scale_row;
+    const unsigned scale_from = (unsigned)(row * scale_row);
+    const unsigned scale_end = (unsigned)scale_row - 8;
+    u32x2 held;
+    auto load_scales = [&](unsigned slice) {
+        const unsigned at = slice * 8 < scale_end ? slice * 8 : scale_end;
+        held = *reinterpret_cast<const u32x2 *>(sbase + (scale_from + at));
+    };
+    // Steps behind the last get scales of 2^-127 on both sides, whose products
+    // vanish: the loop runs over whole pairs of slices.
+    auto store_scales = [&](unsigned slice, int *scales) {
+        unsigned one = held[0], two = held[1];
+        if (slice * 8 > scale_end) {  // uniform: a row's end, read four bytes early
+            one = slice * 8 - scale_end == 4 ? two : 0;
+            two = 0;
+        }
+        scales[(t >> 6) * 128 + lane] = turned(one, part);
+        scales[(t >> 6) * 128 + 64 + lane] = turned(two, part);
+    };
+    const int row_x = wm * MT * 16, row_w = BM + wn * NT * 16;
+    const int lane_row = low * kSliceBytes, slot = (part ^ (low & 7)) * 16;
+    auto read = [&](const unsigned char *codes, const int *scales, int s, Operands<MT, NT> &o) {
+        read_step<MT, NT>(codes + lane_row + (slot ^ (s * 64)), scales + s * 64 + lane, row_x,
+                          row_w, o);
+    };
+    Operands<MT, NT> even, odd;
+    auto turn = [&](unsigned slice, unsigned char *codes, int *scales, unsigned char *codes_next,
+                    int *scales_next) {
+        store_scales(slice + 1, scales_next);
+        read(codes, scales, 1, odd);
+        multiply<MT, NT>(even, acc);
+#pragma unroll
+        for (int i = 0; i < kReads; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
+        }
+        arrive();
+        load_scales(slice + 2);
+        load(slice + 2, codes);
+        read(codes_next, scales_next, 0, even);
+        multiply<MT, NT>(odd, acc);
+#pragma unroll
+        for (int i = 0; i < kLoads + 2; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x010, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        }
+#pragma unroll
+        for (int i = 0; i < kReads; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    load_scales(0);
+    load(0, codes0);
+    store_scales(0, scales0);
+    load_scales(1);
+    arrive();
+    read(codes0, scales0, 0, even);
+    load(1, codes1);
+    const unsigned steps = (unsigned)(a.kp / kPad);
+    for (unsigned slice = 0; 2 * slice < steps; slice += 2) {
+        turn(slice, codes0, scales0, codes1, scales1);
+        turn(slice + 1, codes1, scales1, codes0, scales0);
+    }
+    arrive();
+
+    // Sums through LDS, so that a thread finishes eight columns of its own,
+    // the same for all its rows: kPass rows of the tile at a time.
+    constexpr int kPitch = BN + 4;
+    constexpr int kPassTiles = pass_tiles(MT, WM * 16 * kPitch * 4, sizeof(codes0));
+    constexpr int kPass = kPassTiles * WM * 16, kSweep = kThreads * 8 / BN;
+    const int c = t % (BN / 8) * 8;
+    const size_t n1 = n0 + c;
+    float bias[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        bias[i] = a.bias && n1 + i < a.n ? a.bias[w_first + n1 + i] : 0.0f;
+#pragma unroll
+    for (int j0 = 0; j0 < MT; j0 += kPassTiles) {
+        // The arrays in turn: a pass is read before the next but one is written.
+        float *sums = reinterpret_cast<float *>(j0 / kPassTiles % 2 ? codes1 : codes0);
+#pragma unroll
+        for (int j = 0; j < kPassTiles; ++j)
+#pragma unroll
+            for (int i = 0; i < NT; ++i)
+                *reinterpret_cast<f32x4 *>(sums + ((wm * kPassTiles + j) * 16 + low) * kPitch +
+                                           (wn * NT + i) * 16 + part * 4) = acc[i][j0 + j];
+        __syncthreads();
+        if (n1 >= a.n) continue;
+#pragma unroll 4
+        for (int row = t / (BN / 8); row < kPass; row += kSweep) {
+            const int in = row / (kPassTiles * 16) * (MT * 16) + j0 * 16 + row % (kPassTiles * 16);
+            const f32x4 lo = *reinterpret_cast<const f32x4 *>(sums + row * kPitch + c);
+            const f32x4 hi = *reinterpret_cast<const f32x4 *>(sums + row * kPitch + c + 4);
+            const float scale = scale_of_row[in];
+            const bool real = real_row[in];
+            float v[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float z = (i < 4 ? lo[i & 3] : hi[i & 3]) + bias[i];
+                v[i] = real ? act_of<kFine<T>>(z, ACT) * scale : 0.0f;
             }
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-                for (int j = 0; j < 2; ++j)
-                    acc[i][j] = step16(w[i], sw[i], x[j], sx[j], acc[i][j]);
+            if (in < height) store8<T>(a, m0 + in, n1, v);
         }
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-        const size_t r = m0 + j * 16 + low;
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const size_t c = n0 + i * 16 + part * 4;
-            if (r < rt.r1 && c < a.n) store4<T>(a, rt.expert, real[j], r, c, acc[i][j]);
-        }
+    }
+}
+
+// Rows and columns of a workgroup's tile, by shape.
+struct TileSize {
+    int rows, columns;
+};
+constexpr TileSize kTiles[] = {{16, 16}, {32, 16}, {64, 16}, {128, 128}, {256, 256}};
+enum { kFew1, kFew2, kFew4, kMiddle, kLarge };
+
+size_t tiles_of(const ProductArgs &a, int shape) {
+    const TileSize t = kTiles[shape];
+    // Every run of rows may end within a tile.
+    const size_t high = (a.m + t.rows - 1) / t.rows + (a.offsets ? a.experts + 2 : 0);
+    return high * ((a.n + t.columns - 1) / t.columns);
+}
+
+// Measured (us; large / middle / few rows with 4, 2 and 1 row tiles; bf16 out):
+//   m 16,384 n 4,096 k 4,096: 188 / 270 / 2,230 / 2,675 / -
+//   m  8,192 n 2,048 k 1,024: 20.3 / 25.8 / 197 / 209 / 260     (256 large tiles)
+//   m 16,384 n   512 k   512: 15.1 / 12.0 / 55 / 63 / 92        (128 large tiles)
+//   m    320 n 2,048 k 2,048: 19.3 / 12.0 / 18.6 / 17.3 / 23.0
+//   m    128 n 4,096 k 4,096: 28.3 / 18.7 / 21.7 / 25.1 / 32.1
+//   m     64 n 4,096 k 4,096: 26.9 / 17.3 / 12.7 / 14.4 / 17.8
+//   m     64 n 1,024 k 1,024: 12.0 / 7.9 / 6.1 / 5.0 / 4.3
+//   m     10 n 2,048 k 2,048: 16.3 / 10.1 / 5.7 / 5.2 / 4.9
+// So: staged tiles where the output has more than 2^18 values (a lone staged
+// tile takes about 0.7 us for 256 values of k, the few-row kernel about 3 ns
+// for a thousand outputs) and experts fill more than a quarter of a middle
+// tile; large ones, one to a CU, or middle ones, two to a CU, by what a round
+// of them takes, 8.2 + 2.4 and 4.3 + 1.8 us for each slice of k (from the
+// lines above).  Else as many row tiles as leave a workgroup to every CU.
+int shape_for(const ProductArgs &a) {
+    // The staged kernels address a matrix with 32 bits from a tile's first row
+    // (from the first of all where rows are gathered) and read whole slices.
+    const size_t code_row = a.kp / 2, reach = 0xffffffffu / code_row;
+    const bool staged = a.kp >= kSlice && reach >= 256 && (!a.rows || a.a_rows <= reach);
+    const size_t per = a.m / a.experts;
+    if (staged && per > 32 && a.m * a.n > (1 << 18)) {
+        // Half of the runs of rows end within a tile of their own, about.
+        const size_t slices = (a.kp + kSlice - 1) / kSlice, ends = a.experts / 2;
+        const size_t large = ((a.m + 255) / 256 + ends) * ((a.n + 255) / 256);
+        const size_t middle = ((a.m + 127) / 128 + ends) * ((a.n + 127) / 128);
+        return (large + 255) / 256 * (82 + 24 * slices) <= (middle + 511) / 512 * (43 + 18 * slices)
+                   ? kLarge
+                   : kMiddle;
+    }
+    if (per > 32 && tiles_of(a, kFew4) >= 256) return kFew4;
+    if (per > 16 && tiles_of(a, kFew2) >= 256) return kFew2;
+    return kFew1;
+}
+
+template <class T, int WM, int WN, int MT, int NT>
+void launch_tile(const ProductArgs &a, unsigned tiles, hipStream_t q) {
+    constexpr int threads = 64 * WM * WN;
+    if (a.act == TB_HIP_ACT_NONE)
+        tile_kernel<T, TB_HIP_ACT_NONE, WM, WN, MT, NT><<<tiles, threads, 0, q>>>(a);
+    else if (a.act == TB_HIP_ACT_SILU)
+        tile_kernel<T, TB_HIP_ACT_SILU, WM, WN, MT, NT><<<tiles, threads, 0, q>>>(a);
+    else
+        tile_kernel<T, TB_HIP_ACT_GELU, WM, WN, MT, NT><<<tiles, threads, 0, q>>>(a);
+}
+
+template <class T>
+void launch_product(const ProductArgs &a, int shape, unsigned tiles, hipStream_t q) {
+    switch (shape) {
+        case kFew1: few_kernel<T, 1><<<tiles, 64 * kFewWaves, 0, q>>>(a); break;
+        case kFew2: few_kernel<T, 2><<<tiles, 64 * kFewWaves, 0, q>>>(a); break;
+        case kFew4: few_kernel<T, 4><<<tiles, 64 * kFewWaves, 0, q>>>(a); break;
+        case kMiddle: launch_tile<T, 2, 2, 4, 4>(a, tiles, q); break;
+        default: launch_tile<T, 2, 4, 8, 4>(a, tiles, q); break;
     }
 }
 
@@ -392,18 +786,17 @@ extern "C" int tb_hip_mx4_product_device(const void *a_codes, const void *a_scal
     a.kp = padded(k);
     a.experts = experts;
     a.act = act;
-    const size_t four = 4 * type_size(dtype);
-    a.vector = multiple_of(out, four) && n * type_size(dtype) % four == 0;
-    const size_t tiles = ((m + kTile - 1) / kTile + (offsets ? experts + 2 : 0)) *
-                         ((n + kTile - 1) / kTile);
-    if (tiles > 0x7fffffffu) return 0;
+    a.vector = multiple_of(out, 16) && n * type_size(dtype) % 16 == 0;
     hipStream_t q = reinterpret_cast<hipStream_t>(stream);
     (void)hipGetLastError();
+    const int shape = shape_for(a);
+    const size_t tiles = tiles_of(a, shape);
+    if (tiles > kMaxCount) return 0;
     if (dtype == TB_HIP_F32)
-        product_kernel<float><<<(unsigned)tiles, 256, 0, q>>>(a);
+        launch_product<float>(a, shape, (unsigned)tiles, q);
     else if (dtype == TB_HIP_BF16)
-        product_kernel<__bf16><<<(unsigned)tiles, 256, 0, q>>>(a);
+        launch_product<__bf16>(a, shape, (unsigned)tiles, q);
     else
-        product_kernel<_Float16><<<(unsigned)tiles, 256, 0, q>>>(a);
+        launch_product<_Float16>(a, shape, (unsigned)tiles, q);
     return hipGetLastError() == hipSuccess;
 }
