@@ -16,8 +16,9 @@
 // the same.  Sums go lane by lane, then through LDS per wave (or per row
 // where the lanes of a pixel do not divide a wave), always in the same order.
 //
-// Two launches: partial statistics of chunks of pixels, then the elements,
-// each workgroup joining its image's partials first.
+// A slab whose pixels fit the registers of a workgroup is read once.  Larger
+// ones take two launches: partial statistics of chunks of pixels, then the
+// elements, each workgroup joining its image's partials first.
 #include <initializer_list>
 
 #include "layer_math.h"
@@ -46,6 +47,8 @@ struct Shape {
     int fold;         // lanes divide a wave: sums fold within it
     unsigned chunk;   // pixels of a chunk, whole sweeps
     unsigned chunks;
+    int whole;        // the slab's pixels fit whole: vectors a thread holds
+    unsigned spans;   // workgroups that share a slab's images, backward
 };
 
 struct NormArgs {
@@ -63,15 +66,42 @@ struct NormArgs {
     Shape s;
 };
 
+// v of the lane CTRL & 15 to the left within its sixteen, added.
+template <int CTRL>
+__device__ __forceinline__ float plus_rotated(float v) {
+    return v + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(
+                                             0, __builtin_bit_cast(int, v), CTRL, 15, 15, true));
+}
+__device__ __forceinline__ float plus_far(float v, bool far) {
+    const unsigned u = __builtin_bit_cast(unsigned, v);
+    const auto r = far ? __builtin_amdgcn_permlane32_swap(u, u, false, false)
+                       : __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    return __builtin_bit_cast(float, (unsigned)r[0]) + __builtin_bit_cast(float, (unsigned)r[1]);
+}
+
+// Sums over the lanes of a wave that are a multiple of `lanes` apart, lanes a
+// power of two: rotations within sixteen lanes, exchanges between them.
+template <int V>
+__device__ __forceinline__ void fold(float (&v)[V], int lanes) {
+#define TB_FOLD(limit, step)                          \
+    if (lanes <= limit)                               \
+        _Pragma("unroll") for (int i = 0; i < V; ++i) v[i] = step;
+    TB_FOLD(1, plus_rotated<0x121>(v[i]))
+    TB_FOLD(2, plus_rotated<0x122>(v[i]))
+    TB_FOLD(4, plus_rotated<0x124>(v[i]))
+    TB_FOLD(8, plus_rotated<0x128>(v[i]))
+    TB_FOLD(16, plus_far(v[i], false))
+    TB_FOLD(32, plus_far(v[i], true))
+#undef TB_FOLD
+}
+
 // Writes the workgroup's sums of v over the rows that fold within a wave to
 // part[row][channel]; the caller synchronises.
 template <int V>
 __device__ __forceinline__ void row_sums(float (&v)[V], const Shape &s, float *part) {
     const int t = threadIdx.x;
     if (s.fold) {
-        for (int off = s.lanes; off < 64; off *= 2)
-#pragma unroll
-            for (int i = 0; i < V; ++i) v[i] += __shfl_xor(v[i], off);
+        fold(v, s.lanes);
         const int lane = t & 63;
         if (lane < s.lanes)
 #pragma unroll
@@ -87,8 +117,11 @@ __device__ __forceinline__ int part_rows(const Shape &s) {
 }
 
 __device__ __forceinline__ float wave_sum(float v) {
-    for (int off = 32; off; off >>= 1) v += __shfl_xor(v, off);
-    return v;
+    float one[1] = {v};
+    fold(one, 1);
+    // The lanes add in orders of their own: all take the first one's sum.
+    return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(
+                                         __builtin_bit_cast(int, one[0])));
 }
 
 // The sum of part[rows][slab] over all rows and the `per` channels from c0,
@@ -219,7 +252,7 @@ __global__ __launch_bounds__(kMaxThreads) void norm_parts_kernel(NormArgs a) {
 }
 
 // Joins an image's chunks and writes the chunk's elements.
-template <class T, int B>
+template <class T, int B, int ACT>
 __global__ __launch_bounds__(kMaxThreads) void norm_apply_kernel(NormArgs a) {
     typedef Vec<T, B> X;
     constexpr int V = X::n;
@@ -272,7 +305,7 @@ __global__ __launch_bounds__(kMaxThreads) void norm_apply_kernel(NormArgs a) {
                 X::unpack(*reinterpret_cast<const typename X::raw *>(x + p * a.x_pixel), v);
 #pragma unroll
                 for (int i = 0; i < V; ++i)
-                    v[i] = act_of<kFine<T>>(fmaf(v[i] - mean[i], scale[i], shift[i]), a.act);
+                    v[i] = act_of<kFine<T>, ACT>(fmaf(v[i] - mean[i], scale[i], shift[i]));
                 *reinterpret_cast<typename X::raw *>(y + (size_t)p * a.channels * sizeof(T)) =
                     X::pack(v);
             }
@@ -281,35 +314,35 @@ __global__ __launch_bounds__(kMaxThreads) void norm_apply_kernel(NormArgs a) {
     }
 }
 
-// u = dy act'(z) and h of one vector.
-template <class T, int B>
+// u = dy act'(z) and d = x - mean of one vector.
+template <class T, int B, int ACT>
 __device__ __forceinline__ void grad_terms(typename Vec<T, B>::raw xr,
                                            typename Vec<T, B>::raw gr,
                                            const float (&mean)[Vec<T, B>::n],
-                                           const float (&rstd)[Vec<T, B>::n],
-                                           const float (&gamma)[Vec<T, B>::n],
-                                           const float (&beta)[Vec<T, B>::n], int act,
-                                           float (&u)[Vec<T, B>::n], float (&h)[Vec<T, B>::n]) {
-    Vec<T, B>::unpack(xr, h);
+                                           const float (&scale)[Vec<T, B>::n],
+                                           const float (&beta)[Vec<T, B>::n],
+                                           float (&u)[Vec<T, B>::n], float (&d)[Vec<T, B>::n]) {
+    Vec<T, B>::unpack(xr, d);
     Vec<T, B>::unpack(gr, u);
 #pragma unroll
     for (int i = 0; i < Vec<T, B>::n; ++i) {
-        h[i] = (h[i] - mean[i]) * rstd[i];
-        u[i] *= act_slope<kFine<T>>(fmaf(h[i], gamma[i], beta[i]), act);
+        d[i] -= mean[i];
+        if constexpr (ACT != TB_HIP_ACT_NONE)
+            u[i] *= act_slope<kFine<T>, ACT>(fmaf(d[i], scale[i], beta[i]));
     }
 }
 
-// A thread's channels: statistics and parameters.
+// A thread's channels: z = (x - mean) scale + beta, scale = rstd gamma.
 template <int V>
 struct Channels {
-    float mean[V], rstd[V], gamma[V], beta[V];
+    float mean[V], rstd[V], scale[V], beta[V];
     __device__ __forceinline__ void load(const NormArgs &a, size_t image, int c0) {
 #pragma unroll
         for (int i = 0; i < V; ++i) {
             const size_t g = image * a.groups + (c0 + i) / a.per;
             mean[i] = a.mean_in[g];
             rstd[i] = a.rstd_in[g];
-            gamma[i] = a.gamma ? a.gamma[c0 + i] : 1.0f;
+            scale[i] = rstd[i] * (a.gamma ? a.gamma[c0 + i] : 1.0f);
             beta[i] = a.beta ? a.beta[c0 + i] : 0.0f;
         }
     }
@@ -317,7 +350,7 @@ struct Channels {
 
 // The sums of u and u h of every channel over one chunk:
 // parts[(image, chunk)][channel][2].
-template <class T, int B>
+template <class T, int B, int ACT>
 __global__ __launch_bounds__(kMaxThreads) void grad_parts_kernel(NormArgs a) {
     typedef Vec<T, B> X;
     constexpr int V = X::n;
@@ -339,16 +372,19 @@ __global__ __launch_bounds__(kMaxThreads) void grad_parts_kernel(NormArgs a) {
             const char *x = a.x + w.image * a.x_image + (size_t)c0 * sizeof(T);
             const char *dy = a.dy + w.image * a.dy_image + (size_t)c0 * sizeof(T);
             for (unsigned p = w.p0 + row; p < w.p1; p += s.rows) {
-                float u[V], h[V];
-                grad_terms<T, B>(*reinterpret_cast<const typename X::raw *>(x + p * a.x_pixel),
-                                 *reinterpret_cast<const typename X::raw *>(dy + p * a.dy_pixel),
-                                 ch.mean, ch.rstd, ch.gamma, ch.beta, a.act, u, h);
+                float u[V], d[V];
+                grad_terms<T, B, ACT>(
+                    *reinterpret_cast<const typename X::raw *>(x + p * a.x_pixel),
+                    *reinterpret_cast<const typename X::raw *>(dy + p * a.dy_pixel), ch.mean,
+                    ch.scale, ch.beta, u, d);
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
                     su[i] += u[i];
-                    sh[i] = fmaf(u[i], h[i], sh[i]);
+                    sh[i] = fmaf(u[i], d[i], sh[i]);
                 }
             }
+#pragma unroll
+            for (int i = 0; i < V; ++i) sh[i] *= ch.rstd[i];
         }
         row_sums<V>(su, s, part);
         row_sums<V>(sh, s, part2);
@@ -367,7 +403,7 @@ __global__ __launch_bounds__(kMaxThreads) void grad_parts_kernel(NormArgs a) {
     }
 }
 
-template <class T, int B>
+template <class T, int B, int ACT>
 __global__ __launch_bounds__(kMaxThreads) void grad_apply_kernel(NormArgs a) {
     typedef Vec<T, B> X;
     constexpr int V = X::n;
@@ -408,20 +444,240 @@ __global__ __launch_bounds__(kMaxThreads) void grad_apply_kernel(NormArgs a) {
             const char *x = a.x + w.image * a.x_image + (size_t)c0 * sizeof(T);
             const char *dy = a.dy + w.image * a.dy_image + (size_t)c0 * sizeof(T);
             char *dx = a.out + (w.image * a.pixels * a.channels + c0) * sizeof(T);
+            // dx = u rstd gamma - rstd m1 - d rstd^2 m2
+            float less[V], slope[V];
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                less[i] = ch.rstd[i] * m1[lane * V + i];
+                slope[i] = ch.rstd[i] * ch.rstd[i] * m2[lane * V + i];
+            }
             for (unsigned p = w.p0 + row; p < w.p1; p += s.rows) {
-                float u[V], h[V];
-                grad_terms<T, B>(*reinterpret_cast<const typename X::raw *>(x + p * a.x_pixel),
-                                 *reinterpret_cast<const typename X::raw *>(dy + p * a.dy_pixel),
-                                 ch.mean, ch.rstd, ch.gamma, ch.beta, a.act, u, h);
+                float u[V], d[V];
+                grad_terms<T, B, ACT>(
+                    *reinterpret_cast<const typename X::raw *>(x + p * a.x_pixel),
+                    *reinterpret_cast<const typename X::raw *>(dy + p * a.dy_pixel), ch.mean,
+                    ch.scale, ch.beta, u, d);
 #pragma unroll
                 for (int i = 0; i < V; ++i)
-                    u[i] = ch.rstd[i] * (fmaf(u[i], ch.gamma[i], -m1[lane * V + i]) -
-                                         h[i] * m2[lane * V + i]);
+                    u[i] = fmaf(-d[i], slope[i], fmaf(u[i], ch.scale[i], -less[i]));
                 *reinterpret_cast<typename X::raw *>(dx + (size_t)p * a.channels * sizeof(T)) =
                     X::pack(u);
             }
         }
         __syncthreads();
+    }
+}
+
+// Planes whose slab fits the registers of one workgroup: one pass over memory.
+// Every thread holds NV vectors; the means, then the squared deviations, then
+// the elements come from them.
+template <class T, int B, int NV, int ACT>
+__global__ __launch_bounds__(kMaxThreads) void norm_whole_kernel(NormArgs a) {
+    typedef Vec<T, B> X;
+    constexpr int V = X::n;
+    extern __shared__ float lds[];
+    const Shape s = a.s;
+    const int t = threadIdx.x, rows = part_rows(s), wave = t >> 6, waves = blockDim.x >> 6;
+    float *part = lds, *part2 = part + rows * s.slab, *means = part2 + rows * s.slab,
+          *rstds = means + s.slab;
+    const int lane = t % s.lanes, row = t / s.lanes;
+    const size_t items = a.images * s.slabs;
+    const float inverse = 1.0f / ((float)a.pixels * a.per);
+    // Pixels of a thread: row, row + rows, ... below `count` vectors.
+    const int count = row < s.rows && (unsigned)row < a.pixels
+                          ? (int)((a.pixels - row + s.rows - 1) / s.rows) : 0;
+    for (size_t item = blockIdx.x; item < items; item += gridDim.x) {
+        const size_t at = xcd_contiguous(item, items), image = at / s.slabs;
+        const int first = (int)(at - image * s.slabs) * s.slab, c0 = first + lane * V;
+        const char *x = a.x + image * a.x_image + (size_t)c0 * sizeof(T) + row * a.x_pixel;
+        const size_t step = s.rows * a.x_pixel;
+        typename X::raw raw[NV];
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+            if (j < count) raw[j] = *reinterpret_cast<const typename X::raw *>(x + j * step);
+        float sum[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) sum[i] = 0.0f;
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+            if (j < count) {
+                float v[V];
+                X::unpack(raw[j], v);
+#pragma unroll
+                for (int i = 0; i < V; ++i) sum[i] += v[i];
+            }
+        row_sums<V>(sum, s, part);
+        __syncthreads();
+        for (int g = wave; g < s.slab / a.per; g += waves) {
+            const float m = group_sum(part, rows, s.slab, g * a.per, a.per) * inverse;
+            for (int c = t & 63; c < a.per; c += 64) means[g * a.per + c] = m;
+        }
+        __syncthreads();
+        float mean[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            mean[i] = means[lane * V + i];
+            sum[i] = 0.0f;
+        }
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+            if (j < count) {
+                float v[V];
+                X::unpack(raw[j], v);
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    const float d = v[i] - mean[i];
+                    sum[i] = fmaf(d, d, sum[i]);
+                }
+            }
+        row_sums<V>(sum, s, part2);
+        __syncthreads();
+        for (int g = wave; g < s.slab / a.per; g += waves) {
+            const float var = group_sum(part2, rows, s.slab, g * a.per, a.per) * inverse;
+            const float rstd = 1.0f / sqrtf(var + a.eps);
+            for (int c = t & 63; c < a.per; c += 64) rstds[g * a.per + c] = rstd;
+            if ((t & 63) == 0) {
+                const size_t to = image * a.groups + first / a.per + g;
+                if (a.mean) a.mean[to] = means[g * a.per];
+                if (a.rstd) a.rstd[to] = rstd;
+            }
+        }
+        __syncthreads();
+        float scale[V], shift[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            scale[i] = rstds[lane * V + i] * (count && a.gamma ? a.gamma[c0 + i] : 1.0f);
+            shift[i] = count && a.beta ? a.beta[c0 + i] : 0.0f;
+        }
+        char *y = a.out + ((image * a.pixels + row) * a.channels + c0) * sizeof(T);
+        const size_t out_step = (size_t)s.rows * a.channels * sizeof(T);
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+            if (j < count) {
+                float v[V];
+                X::unpack(raw[j], v);
+#pragma unroll
+                for (int i = 0; i < V; ++i)
+                    v[i] = act_of<kFine<T>, ACT>(fmaf(v[i] - mean[i], scale[i], shift[i]));
+                *reinterpret_cast<typename X::raw *>(y + j * out_step) = X::pack(v);
+            }
+    }
+}
+
+// The backward pass of such planes: x and dy stay in registers between the
+// sums and the elements.  A workgroup takes every so manieth image of its slab
+// and keeps its channels' sums: parts[workgroup of the slab][channel][2].
+// What belongs to a channel is formed by one thread and read from LDS.
+template <class T, int B, int NV, int ACT>
+__global__ __launch_bounds__(kMaxThreads) void grad_whole_kernel(NormArgs a) {
+    typedef Vec<T, B> X;
+    constexpr int V = X::n;
+    extern __shared__ float lds[];
+    const Shape s = a.s;
+    const int t = threadIdx.x, rows = part_rows(s), wave = t >> 6, waves = blockDim.x >> 6;
+    float *part = lds, *part2 = part + rows * s.slab, *m1 = part2 + rows * s.slab,
+          *m2 = m1 + s.slab, *all1 = m2 + s.slab, *all2 = all1 + s.slab, *means = all2 + s.slab,
+          *rstds = means + s.slab, *scales = rstds + s.slab;
+    const int lane = t % s.lanes, row = t / s.lanes;
+    const float inverse = 1.0f / ((float)a.pixels * a.per);
+    const int count = row < s.rows && (unsigned)row < a.pixels
+                          ? (int)((a.pixels - row + s.rows - 1) / s.rows) : 0;
+    const unsigned at = (unsigned)xcd_contiguous(blockIdx.x, gridDim.x), spans = gridDim.x / s.slabs;
+    const int first = (int)(at % s.slabs) * s.slab, c0 = first + lane * V;
+    float beta[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) beta[i] = count && a.beta ? a.beta[c0 + i] : 0.0f;
+    for (int c = t; c < s.slab; c += blockDim.x) all1[c] = all2[c] = 0.0f;
+    for (size_t image = at / s.slabs; image < a.images; image += spans) {
+        const char *x = a.x + image * a.x_image + (size_t)c0 * sizeof(T) + row * a.x_pixel;
+        const char *dy = a.dy + image * a.dy_image + (size_t)c0 * sizeof(T) + row * a.dy_pixel;
+        const size_t x_step = s.rows * a.x_pixel, dy_step = s.rows * a.dy_pixel;
+        typename X::raw xr[NV], gr[NV];
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+            if (j < count) {
+                xr[j] = *reinterpret_cast<const typename X::raw *>(x + j * x_step);
+                gr[j] = *reinterpret_cast<const typename X::raw *>(dy + j * dy_step);
+            }
+        for (int c = t; c < s.slab; c += blockDim.x) {
+            const size_t g = image * a.groups + (first + c) / a.per;
+            const float rstd = a.rstd_in[g];
+            means[c] = a.mean_in[g];
+            rstds[c] = rstd;
+            scales[c] = a.gamma ? rstd * a.gamma[first + c] : rstd;
+        }
+        __syncthreads();
+        float mean[V], scale[V], su[V], sh[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            mean[i] = means[lane * V + i];
+            scale[i] = scales[lane * V + i];
+            su[i] = sh[i] = 0.0f;
+        }
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+            if (j < count) {
+                float u[V], d[V];
+                grad_terms<T, B, ACT>(xr[j], gr[j], mean, scale, beta, u, d);
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    su[i] += u[i];
+                    sh[i] = fmaf(u[i], d[i], sh[i]);
+                }
+            }
+        row_sums<V>(su, s, part);
+        row_sums<V>(sh, s, part2);
+        __syncthreads();
+        for (int c = t; c < s.slab; c += blockDim.x) {
+            float one = 0.0f, two = 0.0f;
+            for (int r = 0; r < rows; ++r) {
+                one += part[r * s.slab + c];
+                two += part2[r * s.slab + c];
+            }
+            two *= rstds[c];
+            all1[c] += one;
+            all2[c] += two;
+            const float gamma = a.gamma ? a.gamma[first + c] : 1.0f;
+            m1[c] = one * gamma;
+            m2[c] = two * gamma;
+        }
+        __syncthreads();
+        // dx = u rstd gamma - rstd m1 - d rstd^2 m2
+        for (int g = wave; g < s.slab / a.per; g += waves) {
+            const float rstd = rstds[g * a.per] * inverse;
+            const float one = group_sum(m1, 1, s.slab, g * a.per, a.per) * rstd;
+            const float two = group_sum(m2, 1, s.slab, g * a.per, a.per) * rstd * rstds[g * a.per];
+            for (int c = t & 63; c < a.per; c += 64) {
+                m1[g * a.per + c] = one;
+                m2[g * a.per + c] = two;
+            }
+        }
+        __syncthreads();
+        float less[V], slope[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            less[i] = m1[lane * V + i];
+            slope[i] = m2[lane * V + i];
+        }
+        char *dx = a.out + ((image * a.pixels + row) * a.channels + c0) * sizeof(T);
+        const size_t out_step = (size_t)s.rows * a.channels * sizeof(T);
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+            if (j < count) {
+                float u[V], d[V];
+                grad_terms<T, B, ACT>(xr[j], gr[j], mean, scale, beta, u, d);
+#pragma unroll
+                for (int i = 0; i < V; ++i)
+                    u[i] = fmaf(-d[i], slope[i], fmaf(u[i], scale[i], -less[i]));
+                *reinterpret_cast<typename X::raw *>(dx + j * out_step) = X::pack(u);
+            }
+        // The next image's tables, sums and means are each written at least
+        // one barrier after their last reads here.
+    }
+    for (int c = t; c < s.slab; c += blockDim.x) {
+        float *to = a.parts + ((size_t)(at / s.slabs) * a.channels + first + c) * 2;
+        to[0] = all1[c];
+        to[1] = all2[c];
     }
 }
 
@@ -466,37 +722,93 @@ __global__ __launch_bounds__(kSumChannels *kSumRows) void grad_sum_kernel(
 
 // --------------------------------------------------------------------------
 
-// The slab is the fewest whole groups whose vectors fill 64-byte runs, with
-// lanes that divide a wave where there are such.  Vectors are 16 bytes, 4 or
-// one element, by what the strides, the channels and the addresses allow.
-Shape shape_of(size_t align, size_t pixels, int channels, int groups, int size) {
-    Shape s = {};
-    const int per = channels / groups;
-    const int widths[3] = {16, 4, size};
+// A slab is whole groups; its vectors are `widest` bytes, 4 or one element, by
+// what the strides, the channels and the addresses allow.  f(bytes, slab,
+// lanes) sees the slabs of the widest vectors that give any.
+template <class F>
+void slabs_of(size_t align, int widest, int channels, int groups, int size, F f) {
+    const int per = channels / groups, widths[3] = {widest, 4, size};
     for (int bytes : widths) {
         if (bytes < size || align % bytes || (size_t)channels * size % bytes) continue;
         const int v = bytes / size;
-        int best = 1 << 30;
-        for (int n = 1; n <= groups; ++n) {
-            const int slab = n * per;
-            if (slab > kMaxSlab) break;
-            if (groups % n || slab % v || slab / v > kMaxThreads) continue;
-            const int lanes = slab / v, run = slab * size;
-            int cost = run < 64 ? 64 / run : run / 64;
-            if (lanes > 64 || 64 % lanes) cost += 16;
-            if (cost < best) {
-                best = cost;
-                s.bytes = bytes;
-                s.slab = slab;
-                s.lanes = lanes;
+        bool any = false;
+        for (int n = 1; n <= groups && n * per <= kMaxSlab; ++n)
+            if (groups % n == 0 && n * per % v == 0 && n * per / v <= kMaxThreads) {
+                any = true;
+                f(bytes, n * per, n * per / v);
             }
-        }
-        if (s.slab) break;
+        if (any) return;
     }
+}
+
+// The most vectors a thread holds: 128 bytes of x, and of dy.
+constexpr int held_most(int bytes) { return bytes == 16 ? 8 : 16; }
+
+int log2_up(size_t n) {
+    int bits = 0;
+    while (((size_t)1 << bits) < n) ++bits;
+    return bits;
+}
+
+bool divides_wave(int lanes) { return lanes <= 64 && 64 % lanes == 0; }
+
+// Slabs that fit the registers of a workgroup: of them the one that fills
+// cache lines and CUs best.  A workgroup too few costs more than a run of half
+// a line, lanes that do not divide a wave more than both.  Vectors are four
+// values: eight of 16 bits would take as many registers for a channel's
+// statistics and parameters as for the data.
+bool whole_shape(Shape &s, size_t align, size_t images, size_t pixels, int channels, int groups,
+                 int size) {
+    int best = 1 << 30;
+    slabs_of(align, 4 * size, channels, groups, size, [&](int bytes, int slab, int lanes) {
+        if (bytes < 4 || (size_t)(kMaxThreads / lanes) * held_most(bytes) < pixels) return;
+        const size_t work = images * (channels / slab);
+        const int run = slab * size;
+        int cost = divides_wave(lanes) ? 0 : 16;
+        if (work < 256) cost += 4 * log2_up((256 + work - 1) / work);
+        if (run < 128) cost += 3 * log2_up((128 + run - 1) / run);
+        if (cost >= best) return;
+        best = cost;
+        s.bytes = bytes;
+        s.slab = slab;
+        s.lanes = lanes;
+    });
+    if (best == 1 << 30) return false;
+    s.slabs = channels / s.slab;
+    // Few workgroups: more threads with fewer vectors each.
+    const int most = held_most(s.bytes);
+    s.whole = images * s.slabs < 512 && (size_t)(kMaxThreads / s.lanes) * 4 >= pixels ? 4 : most;
+    const size_t need = ((pixels + s.whole - 1) / s.whole * s.lanes + 63) / 64 * 64;
+    s.threads = (int)(need < (size_t)kMaxThreads ? need : kMaxThreads);
+    s.rows = s.threads / s.lanes;
+    s.fold = divides_wave(s.lanes);
+    s.chunk = (unsigned)pixels;
+    s.chunks = 1;
+    // Backward: two workgroups of 1,024 threads to a CU, or as many threads.
+    const size_t at_once = 512 * (size_t)(kMaxThreads / s.threads);
+    const size_t spans = (at_once + s.slabs - 1) / s.slabs;
+    s.spans = (unsigned)(spans < images ? spans : images);
+    return true;
+}
+
+// Else slabs of at least 64-byte runs, in chunks of pixels.
+Shape shape_of(size_t align, size_t images, size_t pixels, int channels, int groups, int size) {
+    Shape s = {};
+    if (whole_shape(s, align, images, pixels, channels, groups, size)) return s;
+    int best = 1 << 30;
+    slabs_of(align, 16, channels, groups, size, [&](int bytes, int slab, int lanes) {
+        const int run = slab * size;
+        const int cost = (run < 64 ? 64 / run : run / 64) + (divides_wave(lanes) ? 0 : 16);
+        if (cost >= best) return;
+        best = cost;
+        s.bytes = bytes;
+        s.slab = slab;
+        s.lanes = lanes;
+    });
     s.slabs = channels / s.slab;
     s.threads = s.lanes > kThreads ? kMaxThreads : kThreads;
     s.rows = s.threads / s.lanes;
-    s.fold = s.lanes <= 64 && 64 % s.lanes == 0;
+    s.fold = divides_wave(s.lanes);
     const size_t sweep = (size_t)s.rows * kVectors;
     size_t sweeps = (pixels + sweep - 1) / sweep;
     sweeps = (sweeps + kMaxChunks - 1) / kMaxChunks;
@@ -507,64 +819,97 @@ Shape shape_of(size_t align, size_t pixels, int channels, int groups, int size) 
 
 bool sizes_ok(size_t images, size_t pixels, int channels, int groups, int dtype) {
     return images && images <= kMaxCount && pixels && pixels <= kMaxCount && channels > 0 &&
-           channels <= TB_HIP_NORM_MAX_CHANNELS && groups > 0 && channels % groups == 0 && channels / groups <= TB_HIP_NORM_MAX_GROUP &&
-           known_type(dtype);
+           channels <= TB_HIP_NORM_MAX_CHANNELS && groups > 0 && channels % groups == 0 &&
+           channels / groups <= TB_HIP_NORM_MAX_GROUP && known_type(dtype);
 }
 
 // Rows of the second level of the parameters' sums.
 constexpr size_t kSumSpans = 128, kSumDirect = 1024;
 
-size_t part_bytes(size_t images, const Shape &s, int columns) {
-    return images * s.chunks * columns * 2 * sizeof(float);
-}
+// Rows of the channels' partial sums, backward.
+size_t sum_rows(size_t images, const Shape &s) { return s.whole ? s.spans : images * s.chunks; }
 
 size_t grid_of(const NormArgs &a) {
     const size_t items = a.images * a.s.slabs * a.s.chunks;
     return items < kMaxGrid ? items : kMaxGrid;
 }
 
-template <class T, int B>
-void forward(const NormArgs &a, hipStream_t q) {
+size_t part_floats(const Shape &s) { return (size_t)(s.fold ? s.threads / 64 : s.rows) * s.slab; }
+
+template <class T, int B, int ACT>
+void launch_forward(const NormArgs &a, hipStream_t q) {
     const Shape &s = a.s;
-    const int rows = s.fold ? s.threads / 64 : s.rows;
-    const size_t lds = ((size_t)rows * s.slab + 3 * s.slab) * sizeof(float);
-    norm_parts_kernel<T, B><<<(unsigned)grid_of(a), s.threads, lds, q>>>(a);
-    norm_apply_kernel<T, B>
-        <<<(unsigned)grid_of(a), s.threads, 2 * s.slab * sizeof(float), q>>>(a);
+    const size_t part = part_floats(s) * sizeof(float), slab = s.slab * sizeof(float);
+    const unsigned grid = (unsigned)grid_of(a);
+    if constexpr (B == 4 * sizeof(T) || B == 4) {
+        constexpr int most = held_most(B);
+        if (s.whole == 4)
+            norm_whole_kernel<T, B, 4, ACT><<<grid, s.threads, 2 * part + 2 * slab, q>>>(a);
+        if (s.whole == most)
+            norm_whole_kernel<T, B, most, ACT><<<grid, s.threads, 2 * part + 2 * slab, q>>>(a);
+        if (s.whole) return;
+    }
+    if constexpr (B != 8) {
+        norm_parts_kernel<T, B><<<grid, s.threads, part + 3 * slab, q>>>(a);
+        norm_apply_kernel<T, B, ACT><<<grid, s.threads, 2 * slab, q>>>(a);
+    }
 }
 
-template <class T, int B>
-void backward(const NormArgs &a, hipStream_t q) {
+template <class T, int B, int ACT>
+void launch_backward(const NormArgs &a, hipStream_t q) {
     const Shape &s = a.s;
-    const int rows = s.fold ? s.threads / 64 : s.rows;
-    grad_parts_kernel<T, B>
-        <<<(unsigned)grid_of(a), s.threads, (size_t)2 * rows * s.slab * sizeof(float), q>>>(a);
-    grad_apply_kernel<T, B>
-        <<<(unsigned)grid_of(a), s.threads, 2 * s.slab * sizeof(float), q>>>(a);
+    const size_t part = part_floats(s) * sizeof(float), slab = s.slab * sizeof(float);
+    if constexpr (B == 4 * sizeof(T) || B == 4) {
+        constexpr int most = held_most(B);
+        const unsigned grid = s.spans * s.slabs;
+        if (s.whole == 4)
+            grad_whole_kernel<T, B, 4, ACT><<<grid, s.threads, 2 * part + 7 * slab, q>>>(a);
+        if (s.whole == most)
+            grad_whole_kernel<T, B, most, ACT><<<grid, s.threads, 2 * part + 7 * slab, q>>>(a);
+        if (s.whole) return;
+    }
+    if constexpr (B != 8) {
+        const unsigned grid = (unsigned)grid_of(a);
+        grad_parts_kernel<T, B, ACT><<<grid, s.threads, 2 * part, q>>>(a);
+        grad_apply_kernel<T, B, ACT><<<grid, s.threads, 2 * slab, q>>>(a);
+    }
 }
 
 struct Forward {
-    template <class T, int B>
-    static void run(const NormArgs &a, hipStream_t q) { forward<T, B>(a, q); }
+    template <class T, int B, int ACT>
+    static void run(const NormArgs &a, hipStream_t q) { launch_forward<T, B, ACT>(a, q); }
 };
 struct Backward {
-    template <class T, int B>
-    static void run(const NormArgs &a, hipStream_t q) { backward<T, B>(a, q); }
+    template <class T, int B, int ACT>
+    static void run(const NormArgs &a, hipStream_t q) { launch_backward<T, B, ACT>(a, q); }
 };
+
+template <class F, class T>
+void by_width(const NormArgs &a, hipStream_t q) {
+    with_act(a.act, [&](auto act) {
+        constexpr int ACT = decltype(act)::value;
+        switch (a.s.bytes) {
+            case 16: F::template run<T, 16, ACT>(a, q); break;
+            case 4: F::template run<T, 4, ACT>(a, q); break;
+            default:
+                if constexpr (sizeof(T) == 2) {
+                    if (a.s.bytes == 8)
+                        F::template run<T, 8, ACT>(a, q);
+                    else
+                        F::template run<T, 2, ACT>(a, q);
+                }
+        }
+    });
+}
 
 template <class F>
 void dispatch(const NormArgs &a, int dtype, hipStream_t q) {
-    const int b = a.s.bytes;
     if (dtype == TB_HIP_F32)
-        b == 16 ? F::template run<float, 16>(a, q) : F::template run<float, 4>(a, q);
+        by_width<F, float>(a, q);
     else if (dtype == TB_HIP_BF16)
-        b == 16  ? F::template run<__bf16, 16>(a, q)
-        : b == 4 ? F::template run<__bf16, 4>(a, q)
-                 : F::template run<__bf16, 2>(a, q);
+        by_width<F, __bf16>(a, q);
     else
-        b == 16  ? F::template run<_Float16, 16>(a, q)
-        : b == 4 ? F::template run<_Float16, 4>(a, q)
-                 : F::template run<_Float16, 2>(a, q);
+        by_width<F, _Float16>(a, q);
 }
 
 // The common alignment of the addresses and strides.
@@ -583,13 +928,13 @@ extern "C" size_t tb_hip_group_norm_workspace_bytes(size_t images, size_t pixels
     if (!sizes_ok(images, pixels, channels, groups, dtype)) return 0;
     const int size = type_size(dtype);
     size_t most = 0;
-    for (size_t align : {size_t(16), size_t(4), size_t(size)}) {
-        const Shape s = shape_of(align, pixels, channels, groups, size);
-        const size_t need = backward ? part_bytes(images, s, channels) +
-                                           kSumSpans * channels * 2 * sizeof(float)
-                                     : part_bytes(images, s, groups);
+    for (size_t align : {size_t(16), size_t(8), size_t(4), size_t(size)}) {
+        const Shape s = shape_of(align, images, pixels, channels, groups, size);
+        const size_t need =
+            backward ? (sum_rows(images, s) + kSumSpans) * channels : images * s.chunks * groups;
         most = need > most ? need : most;
     }
+    most *= 2 * sizeof(float);
     return (most + 15) & ~size_t(15);
 }
 
@@ -621,7 +966,7 @@ extern "C" int tb_hip_group_norm_device(const void *x, size_t image_stride, size
     a.per = channels / groups;
     a.eps = eps;
     a.act = act;
-    a.s = shape_of(align, pixels, channels, groups, size);
+    a.s = shape_of(align, images, pixels, channels, groups, size);
     (void)hipGetLastError();
     dispatch<Forward>(a, dtype, reinterpret_cast<hipStream_t>(stream));
     return hipGetLastError() == hipSuccess;
@@ -660,14 +1005,14 @@ extern "C" int tb_hip_group_norm_backward_device(
     a.groups = groups;
     a.per = channels / groups;
     a.act = act;
-    a.s = shape_of(align, pixels, channels, groups, size);
+    a.s = shape_of(align, images, pixels, channels, groups, size);
     hipStream_t q = reinterpret_cast<hipStream_t>(stream);
     (void)hipGetLastError();
     dispatch<Backward>(a, dtype, q);
     if (dgamma) {
         const unsigned tiles = (unsigned)((channels + kSumChannels - 1) / kSumChannels);
         const float *parts = a.parts;
-        size_t rows = images * a.s.chunks;
+        size_t rows = sum_rows(images, a.s);
         if (rows > kSumDirect) {
             float *next = a.parts + rows * channels * 2;
             grad_sum_kernel<<<dim3(tiles, kSumSpans), kSumChannels * kSumRows, 0, q>>>(

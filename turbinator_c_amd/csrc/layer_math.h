@@ -73,24 +73,40 @@ __device__ __forceinline__ float sigmoid_of(float z) {
     return d < 0x1p126f ? fmaf(fmaf(-d, q, 1.0f), q, q) : q;
 }
 
-template <bool FINE>
-__device__ __forceinline__ float act_of(float z, int act) {
-    if (act == TB_HIP_ACT_SILU) return z * sigmoid_of<FINE>(z);
-    if (act == TB_HIP_ACT_GELU) return 0.5f * z * (1.0f + erff(z * 0.70710678118654752440f));
+template <bool FINE, int ACT>
+__device__ __forceinline__ float act_of(float z) {
+    if constexpr (ACT == TB_HIP_ACT_SILU) return z * sigmoid_of<FINE>(z);
+    if constexpr (ACT == TB_HIP_ACT_GELU)
+        return 0.5f * z * (1.0f + erff(z * 0.70710678118654752440f));
     return z;
 }
 
 // The derivative of act_of.
-template <bool FINE>
-__device__ __forceinline__ float act_slope(float z, int act) {
-    if (act == TB_HIP_ACT_SILU) {
+template <bool FINE, int ACT>
+__device__ __forceinline__ float act_slope(float z) {
+    if constexpr (ACT == TB_HIP_ACT_SILU) {
         const float s = sigmoid_of<FINE>(z);
-        return s * fmaf(z, 1.0f - s, 1.0f);
+        return fmaf(z, fmaf(-s, s, s), s);
     }
-    if (act == TB_HIP_ACT_GELU)
+    if constexpr (ACT == TB_HIP_ACT_GELU)
         return 0.5f * (1.0f + erff(z * 0.70710678118654752440f)) +
                z * (0.39894228040143267794f * exp_of<FINE>(-0.5f * z * z));
     return 1.0f;
+}
+
+// Calls f with the activation as a compile-time constant.
+template <int N>
+struct Int {
+    static constexpr int value = N;
+};
+template <class F>
+inline void with_act(int act, F f) {
+    if (act == TB_HIP_ACT_SILU)
+        f(Int<TB_HIP_ACT_SILU>());
+    else if (act == TB_HIP_ACT_GELU)
+        f(Int<TB_HIP_ACT_GELU>());
+    else
+        f(Int<TB_HIP_ACT_NONE>());
 }
 
 template <class T>

@@ -218,7 +218,7 @@ __device__ __forceinline__ f32x4 step16(i32x4 w, int ws, i32x4 x, int xs, f32x4 
 }
 
 // Four consecutive columns n0 .. of row r: bias, activation, row scale.
-template <class T>
+template <class T, int ACT>
 __device__ __forceinline__ void store4(const ProductArgs &a, int expert, bool real, size_t r,
                                        size_t n0, f32x4 c) {
     T *out = reinterpret_cast<T *>(a.out) + r * a.n + n0;
@@ -229,7 +229,7 @@ __device__ __forceinline__ void store4(const ProductArgs &a, int expert, bool re
         v[i] = 0.0f;
         if (real && n0 + i < a.n) {
             const float z = a.bias ? c[i] + a.bias[(size_t)expert * a.n + n0 + i] : c[i];
-            v[i] = act_of<kFine<T>>(z, a.act) * scale;
+            v[i] = act_of<kFine<T>, ACT>(z) * scale;
         }
     }
     if (a.vector && n0 + 4 <= a.n) {
@@ -248,7 +248,7 @@ __device__ __forceinline__ void store4(const ProductArgs &a, int expert, bool re
 // operand, so a lane ends with four consecutive columns of one row.
 constexpr int kFewWaves = 8;
 
-template <class T, int MT>
+template <class T, int ACT, int MT>
 __global__ __launch_bounds__(64 * kFewWaves) void few_kernel(ProductArgs a) {
     __shared__ f32x4 sums[kFewWaves][MT][64];
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
@@ -306,7 +306,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_kernel(ProductArgs a) {
         f32x4 sum = sums[0][j][lane];
         for (int w = 1; w < kFewWaves; ++w) sum += sums[w][j][lane];
         const size_t r = rt.r0 + j * 16 + low, c = n0 + part * 4;
-        if (r < rt.r1 && c < a.n) store4<T>(a, rt.expert, real >> j & 1, r, c, sum);
+        if (r < rt.r1 && c < a.n) store4<T, ACT>(a, rt.expert, real >> j & 1, r, c, sum);
     }
 }
 
@@ -615,7 +615,7 @@ __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(ProductArgs a) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const float z = (i < 4 ? lo[i & 3] : hi[i & 3]) + bias[i];
-                v[i] = real ? act_of<kFine<T>>(z, ACT) * scale : 0.0f;
+                v[i] = real ? act_of<kFine<T>, ACT>(z) * scale : 0.0f;
             }
             if (in < height) store8<T>(a, m0 + in, n1, v);
         }
@@ -671,26 +671,18 @@ int shape_for(const ProductArgs &a) {
     return kFew1;
 }
 
-template <class T, int WM, int WN, int MT, int NT>
-void launch_tile(const ProductArgs &a, unsigned tiles, hipStream_t q) {
-    constexpr int threads = 64 * WM * WN;
-    if (a.act == TB_HIP_ACT_NONE)
-        tile_kernel<T, TB_HIP_ACT_NONE, WM, WN, MT, NT><<<tiles, threads, 0, q>>>(a);
-    else if (a.act == TB_HIP_ACT_SILU)
-        tile_kernel<T, TB_HIP_ACT_SILU, WM, WN, MT, NT><<<tiles, threads, 0, q>>>(a);
-    else
-        tile_kernel<T, TB_HIP_ACT_GELU, WM, WN, MT, NT><<<tiles, threads, 0, q>>>(a);
-}
-
 template <class T>
 void launch_product(const ProductArgs &a, int shape, unsigned tiles, hipStream_t q) {
-    switch (shape) {
-        case kFew1: few_kernel<T, 1><<<tiles, 64 * kFewWaves, 0, q>>>(a); break;
-        case kFew2: few_kernel<T, 2><<<tiles, 64 * kFewWaves, 0, q>>>(a); break;
-        case kFew4: few_kernel<T, 4><<<tiles, 64 * kFewWaves, 0, q>>>(a); break;
-        case kMiddle: launch_tile<T, 2, 2, 4, 4>(a, tiles, q); break;
-        default: launch_tile<T, 2, 4, 8, 4>(a, tiles, q); break;
-    }
+    with_act(a.act, [&](auto act) {
+        constexpr int ACT = decltype(act)::value;
+        switch (shape) {
+            case kFew1: few_kernel<T, ACT, 1><<<tiles, 64 * kFewWaves, 0, q>>>(a); break;
+            case kFew2: few_kernel<T, ACT, 2><<<tiles, 64 * kFewWaves, 0, q>>>(a); break;
+            case kFew4: few_kernel<T, ACT, 4><<<tiles, 64 * kFewWaves, 0, q>>>(a); break;
+            case kMiddle: tile_kernel<T, ACT, 2, 2, 4, 4><<<tiles, 256, 0, q>>>(a); break;
+            default: tile_kernel<T, ACT, 2, 4, 8, 4><<<tiles, 512, 0, q>>>(a); break;
+        }
+    });
 }
 
 unsigned grid_for(size_t items) {
