@@ -752,8 +752,10 @@ int log2_up(size_t n) {
 
 bool divides_wave(int lanes) { return lanes <= 64 && 64 % lanes == 0; }
 
-// Slabs that fit the registers of a workgroup: of them the one that fills
-// cache lines and CUs best.  A workgroup too few costs more than a run of half
+// Slabs that fit the registers of a workgroup: of them the one whose runs are
+// nearest to 64 bytes and that fills the CUs (4,096 x 1,024 x 64 bf16, us:
+// runs of 32 bytes 317, 64 251, 128 289; gradients of 1,024 x 2,048 x 64: 283,
+// 256 and more than the registers).  A workgroup too few costs more than a run of half
 // a line, lanes that do not divide a wave more than both.  Vectors are four
 // values: eight of 16 bits would take as many registers for a channel's
 // statistics and parameters as for the data.
@@ -766,7 +768,7 @@ bool whole_shape(Shape &s, size_t align, size_t images, size_t pixels, int chann
         const int run = slab * size;
         int cost = divides_wave(lanes) ? 0 : 16;
         if (work < 256) cost += 4 * log2_up((256 + work - 1) / work);
-        if (run < 128) cost += 3 * log2_up((128 + run - 1) / run);
+        cost += 3 * (run < 64 ? log2_up((64 + run - 1) / run) : log2_up((run + 63) / 64));
         if (cost >= best) return;
         best = cost;
         s.bytes = bytes;
@@ -784,8 +786,8 @@ bool whole_shape(Shape &s, size_t align, size_t images, size_t pixels, int chann
     s.fold = divides_wave(s.lanes);
     s.chunk = (unsigned)pixels;
     s.chunks = 1;
-    // Backward: two workgroups of 1,024 threads to a CU, or as many threads.
-    const size_t at_once = 512 * (size_t)(kMaxThreads / s.threads);
+    // Backward: one workgroup of 1,024 threads to a CU, or as many threads.
+    const size_t at_once = 256 * (size_t)(kMaxThreads / s.threads);
     const size_t spans = (at_once + s.slabs - 1) / s.slabs;
     s.spans = (unsigned)(spans < images ? spans : images);
     return true;
