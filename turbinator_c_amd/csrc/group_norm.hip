@@ -66,17 +66,14 @@ struct NormArgs {
     Shape s;
 };
 
-// v of the lane CTRL & 15 to the left within its sixteen, added.
-template <int CTRL>
+template <int N>
 __device__ __forceinline__ float plus_rotated(float v) {
-    return v + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(
-                                             0, __builtin_bit_cast(int, v), CTRL, 15, 15, true));
+    return v + __builtin_bit_cast(float, rotated<N>(__builtin_bit_cast(int, v)));
 }
 __device__ __forceinline__ float plus_far(float v, bool far) {
-    const unsigned u = __builtin_bit_cast(unsigned, v);
-    const auto r = far ? __builtin_amdgcn_permlane32_swap(u, u, false, false)
-                       : __builtin_amdgcn_permlane16_swap(u, u, false, false);
-    return __builtin_bit_cast(float, (unsigned)r[0]) + __builtin_bit_cast(float, (unsigned)r[1]);
+    return __builtin_bit_cast(float, across(__builtin_bit_cast(int, v), far, [](int a, int b) {
+        return __builtin_bit_cast(int, __builtin_bit_cast(float, a) + __builtin_bit_cast(float, b));
+    }));
 }
 
 // Sums over the lanes of a wave that are a multiple of `lanes` apart, lanes a
@@ -86,10 +83,10 @@ __device__ __forceinline__ void fold(float (&v)[V], int lanes) {
 #define TB_FOLD(limit, step)                          \
     if (lanes <= limit)                               \
         _Pragma("unroll") for (int i = 0; i < V; ++i) v[i] = step;
-    TB_FOLD(1, plus_rotated<0x121>(v[i]))
-    TB_FOLD(2, plus_rotated<0x122>(v[i]))
-    TB_FOLD(4, plus_rotated<0x124>(v[i]))
-    TB_FOLD(8, plus_rotated<0x128>(v[i]))
+    TB_FOLD(1, plus_rotated<1>(v[i]))
+    TB_FOLD(2, plus_rotated<2>(v[i]))
+    TB_FOLD(4, plus_rotated<4>(v[i]))
+    TB_FOLD(8, plus_rotated<8>(v[i]))
     TB_FOLD(16, plus_far(v[i], false))
     TB_FOLD(32, plus_far(v[i], true))
 #undef TB_FOLD

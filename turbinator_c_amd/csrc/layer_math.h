@@ -52,25 +52,21 @@ constexpr float kLn2 = 0.69314718055994530942f;
 // e^x.  v_exp_f32 is 2^x to 1 ulp; the rounding of x log2(e) alone would cost
 // |x| 2^-24, which a result rounded to 16 bits does not show.  With FINE the
 // product's remainder r is put back as the factor 1 + r ln 2, which keeps
-// about 2 ulp over the whole range.
+// about 2 ulp while e^x and its inverse are normal.
 template <bool FINE>
 __device__ __forceinline__ float exp_of(float x) {
     const float p = x * kLog2e;
     const float e = __builtin_amdgcn_exp2f(p);
     if constexpr (!FINE) return e;
     const float r = fmaf(x, kLog2eLow, fmaf(x, kLog2e, -p));
-    // Past the range of floats e is 0 or inf and r may be NaN or huge.
-    return (p > -150.0f && p < 128.0f) ? fmaf(e, r * kLn2, e) : e;
+    // Further out e may be 0 or inf and r NaN.
+    return __builtin_fabsf(p) < 126.0f ? fmaf(e, r * kLn2, e) : e;
 }
 
-// 1 / (1 + e^-z): v_rcp_f32 is within 1 ulp; FINE adds one Newton step, kept
-// off infinite denominators.
+// 1 / (1 + e^-z); v_rcp_f32 is within 1 ulp.
 template <bool FINE>
 __device__ __forceinline__ float sigmoid_of(float z) {
-    const float d = 1.0f + exp_of<FINE>(-z);
-    const float q = __builtin_amdgcn_rcpf(d);
-    if constexpr (!FINE) return q;
-    return d < 0x1p126f ? fmaf(fmaf(-d, q, 1.0f), q, q) : q;
+    return __builtin_amdgcn_rcpf(1.0f + exp_of<FINE>(-z));
 }
 
 template <bool FINE, int ACT>
@@ -107,6 +103,20 @@ inline void with_act(int act, F f) {
         f(Int<TB_HIP_ACT_GELU>());
     else
         f(Int<TB_HIP_ACT_NONE>());
+}
+
+// The value of the lane `N` to the left within its sixteen lanes, around.
+template <int N>
+__device__ __forceinline__ int rotated(int v) {
+    return __builtin_amdgcn_update_dpp(0, v, 0x120 + N, 15, 15, true);
+}
+
+// f over v and the value of the partner 16 or 32 lanes away.
+template <class F>
+__device__ __forceinline__ int across(int v, bool far, F f) {
+    const auto r = far ? __builtin_amdgcn_permlane32_swap(v, v, false, false)
+                       : __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    return f((int)r[0], (int)r[1]);
 }
 
 template <class T>

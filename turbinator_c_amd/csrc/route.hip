@@ -37,35 +37,51 @@ struct RouteArgs {
     float *weights;
     char *dlogits;
     size_t tokens;
-    int n, k, groups, kept, lanes, score, renorm;
+    int n, k, groups, kept, lanes, score, renorm, vector;
     float scale;
 };
 
-// Floats as unsigned integers of the same order: -0 as +0, NaN above all, and
-// 0 for -inf, which is never chosen.
-__device__ __forceinline__ unsigned key_of(float x) {
-    if (x != x) return 0xffffffffu;
-    const unsigned u = __builtin_bit_cast(unsigned, x + 0.0f);
-    if (u == 0xff800000u) return 0u;
-    return u & 0x80000000u ? ~u : u | 0x80000000u;
+// Floats as integers of the same order: -0 as +0, NaN above all.  kNone and
+// below, -inf and kGone, are never chosen.
+constexpr int kNone = (int)0x807fffff, kGone = (int)0x80000000;
+
+__device__ __forceinline__ int key_of(float x) {
+    const int u = __builtin_bit_cast(int, x + 0.0f);
+    return x != x ? 0x7fffffff : u ^ ((u >> 31) & 0x7fffffff);
+}
+__device__ __forceinline__ float float_of(int key) {
+    return __builtin_bit_cast(float, key ^ ((key >> 31) & 0x7fffffff));
 }
 
+// f over the values of a token's lanes, the same in all of them where f does
+// not depend on the order.
+template <class F>
+__device__ __forceinline__ int over_lanes(int v, int lanes, F f) {
+    // Exchanges within 2, 4 and 8 lanes (mirrors of the groups below them).
+    if (lanes > 1) v = f(v, __builtin_amdgcn_update_dpp(0, v, 0xb1, 15, 15, true));   // quad 1 0 3 2
+    if (lanes > 2) v = f(v, __builtin_amdgcn_update_dpp(0, v, 0x4e, 15, 15, true));   // quad 2 3 0 1
+    if (lanes > 4) v = f(v, __builtin_amdgcn_update_dpp(0, v, 0x141, 15, 15, true));  // half mirror
+    if (lanes > 8) v = f(v, __builtin_amdgcn_update_dpp(0, v, 0x140, 15, 15, true));  // mirror
+    if (lanes > 16) v = across(v, false, f);
+    if (lanes > 32) v = across(v, true, f);
+    return v;
+}
 __device__ __forceinline__ float lanes_max(float v, int lanes) {
-    for (int off = 1; off < lanes; off *= 2) v = fmaxf(v, __shfl_xor(v, off));
-    return v;
+    return __builtin_bit_cast(float, over_lanes(__builtin_bit_cast(int, v), lanes, [](int a, int b) {
+        return __builtin_bit_cast(int, fmaxf(__builtin_bit_cast(float, a), __builtin_bit_cast(float, b)));
+    }));
 }
-
+// The lanes' orders differ, but a pair's sum does not, so neither does theirs.
 __device__ __forceinline__ float lanes_sum(float v, int lanes) {
-    for (int off = 1; off < lanes; off *= 2) v += __shfl_xor(v, off);
-    return v;
+    return __builtin_bit_cast(float, over_lanes(__builtin_bit_cast(int, v), lanes, [](int a, int b) {
+        return __builtin_bit_cast(int, __builtin_bit_cast(float, a) + __builtin_bit_cast(float, b));
+    }));
 }
-
-__device__ __forceinline__ unsigned lanes_max_key(unsigned v, int lanes) {
-    for (int off = 1; off < lanes; off *= 2) {
-        const unsigned o = __shfl_xor(v, off);
-        v = o > v ? o : v;
-    }
-    return v;
+__device__ __forceinline__ int lanes_max_int(int v, int lanes) {
+    return over_lanes(v, lanes, [](int a, int b) { return a > b ? a : b; });
+}
+__device__ __forceinline__ int lanes_min_int(int v, int lanes) {
+    return over_lanes(v, lanes, [](int a, int b) { return a < b ? a : b; });
 }
 
 // LDS that only the calling wave uses: its accesses are in order.
@@ -79,149 +95,171 @@ __device__ __forceinline__ float element(const char *row, int i) {
     return (float)reinterpret_cast<const T *>(row)[i];
 }
 
+// Q consecutive logits, -inf past the last; with `vector` rows start on 16
+// bytes and hold whole vectors.
 template <class T, int Q>
-__device__ __forceinline__ void load_row(const char *row, int e0, int n, float (&x)[Q]) {
+__device__ __forceinline__ void load_row(const char *row, int e0, int n, int vector,
+                                         float (&x)[Q]) {
+    typedef Vec<T, 16> X;
+    if (vector) {
+        if (e0 < n) {
 #pragma unroll
-    for (int j = 0; j < Q; ++j) x[j] = e0 + j < n ? element<T>(row, e0 + j) : -__builtin_inff();
+            for (int p = 0; p < Q / X::n; ++p) {
+                float part[X::n];
+                X::unpack(reinterpret_cast<const typename X::raw *>(row + e0 * sizeof(T))[p],
+                          part);
+#pragma unroll
+                for (int j = 0; j < X::n; ++j) x[p * X::n + j] = part[j];
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < Q; ++j) x[j] = -__builtin_inff();
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < Q; ++j)
+            x[j] = e0 + j < n ? element<T>(row, e0 + j) : -__builtin_inff();
+    }
 }
 
-// Whether v is among the kept highest of all[count], ties to the lower index.
-__device__ __forceinline__ bool in_best(const unsigned *all, int count, int i, int kept) {
-    const unsigned v = all[i];
+// Whether all[i] is among the `kept` highest of all[count], ties to the lower
+// index.
+__device__ __forceinline__ bool in_best(const int *all, int count, int i, int kept) {
+    const int v = all[i];
     int before = 0;
     for (int j = 0; j < count; ++j) before += all[j] > v || (all[j] == v && j < i);
     return before < kept;
 }
 
+// LDS of a token: its picks, with groups also the keys and the groups'
+// standings, one word apart from the next token's so that tokens lie in
+// different banks.
+__host__ __device__ inline int route_words(int span, int k, bool groups) {
+    return (k + (groups ? 2 * span : 0)) | 1;
+}
+
 template <class T, int Q>
 __global__ __launch_bounds__(kThreads) void route_kernel(RouteArgs a) {
-    // Per token: with groups the keys and the groups' standings, then the
-    // picks (a token's span of 8 or more experts or its 32 picks at most).
-    __shared__ unsigned keys[kThreads * Q], stands[kThreads * Q];
-    __shared__ int pick_at[kThreads * 8];
-    __shared__ float pick_s[kThreads * 8];
+    extern __shared__ int lds[];
     const int W = a.lanes, per_block = kThreads / W, t = threadIdx.x;
     const int lane = t & (W - 1), slot = t / W;
     const int e0 = lane * Q, span = W * Q;
-    unsigned *my_keys = keys + slot * span, *my_stands = stands + slot * span;
-    const int picks = span < TB_HIP_ROUTE_MAX_K ? span : TB_HIP_ROUTE_MAX_K;
-    int *at = pick_at + slot * picks;
-    float *ps = pick_s + slot * picks;
-    const unsigned long long mine = (W == 64 ? ~0ull : ((1ull << W) - 1)) << ((t & 63) - lane);
+    const bool grouped = a.kept < a.groups;
+    int *at = lds + slot * route_words(span, a.k, grouped), *keys = at + a.k,
+        *stands = keys + span;
+    const bool soft = a.score == TB_HIP_SCORE_SOFTMAX;
     for (size_t base = (size_t)blockIdx.x * per_block; base < a.tokens;
          base += (size_t)gridDim.x * per_block) {
         const size_t token = base + slot;
         const bool live = token < a.tokens && (!a.valid || a.valid[token]);
-        float x[Q], s[Q];
-        unsigned key[Q];
+        const char *row = a.logits + token * a.stride;
+        float x[Q];
+        int key[Q];
         if (live)
-            load_row<T, Q>(a.logits + token * a.stride, e0, a.n, x);
+            load_row<T, Q>(row, e0, a.n, a.vector, x);
         else
 #pragma unroll
             for (int j = 0; j < Q; ++j) x[j] = -__builtin_inff();
-        float top = -__builtin_inff(), sum = 0.0f;
-        if (a.score == TB_HIP_SCORE_SOFTMAX) {
+        // The row's largest logit and sum, where weights or keys need them.
+        float top = -__builtin_inff(), inverse = 1.0f;
+        if (soft && (a.bias || !a.renorm)) {
+            float sum = 0.0f;
 #pragma unroll
             for (int j = 0; j < Q; ++j) top = fmaxf(top, x[j]);
             top = lanes_max(top, W);
 #pragma unroll
+            for (int j = 0; j < Q; ++j) sum += e0 + j < a.n ? exp_of<true>(x[j] - top) : 0.0f;
+            inverse = 1.0f / lanes_sum(sum, W);
+        }
+#pragma unroll
+        for (int j = 0; j < Q; ++j) key[j] = key_of(x[j]);
+        if (a.bias) {
+#pragma unroll
             for (int j = 0; j < Q; ++j) {
-                s[j] = e0 + j < a.n ? exp_of<true>(x[j] - top) : 0.0f;
-                sum += s[j];
+                const float s = soft ? exp_of<true>(x[j] - top) * inverse : sigmoid_of<true>(x[j]);
+                if (key[j] > kNone) key[j] = key_of(s + a.bias[e0 + j]);
             }
-            const float inverse = 1.0f / lanes_sum(sum, W);
-#pragma unroll
-            for (int j = 0; j < Q; ++j) s[j] *= inverse;
-        } else {
-#pragma unroll
-            for (int j = 0; j < Q; ++j) s[j] = sigmoid_of<true>(x[j]);
         }
-#pragma unroll
-        for (int j = 0; j < Q; ++j) {
-            key[j] = key_of(x[j]);
-            if (a.bias && key[j]) key[j] = key_of(s[j] + a.bias[e0 + j]);
-        }
-        if (a.kept < a.groups) {
+        if (grouped) {
             const int per = a.n / a.groups;
 #pragma unroll
-            for (int j = 0; j < Q; ++j) my_keys[e0 + j] = key[j];
+            for (int j = 0; j < Q; ++j) keys[e0 + j] = key[j];
             wave_fence();
             for (int g = lane; g < a.groups; g += W) {
-                unsigned best = 0, next = 0;
+                int best = kGone, next = kGone;
                 for (int i = 0; i < per; ++i) {
-                    const unsigned v = my_keys[g * per + i];
-                    next = v > best ? best : v > next ? v : next;
+                    const int v = keys[g * per + i], low = v < best ? v : best;
+                    next = low > next ? low : next;
                     best = v > best ? v : best;
                 }
-                if (a.bias && next) {
-                    // Back to floats; NaN keys stay above all.
-                    const unsigned b = best & 0x80000000u ? best & 0x7fffffffu : ~best;
-                    const unsigned c = next & 0x80000000u ? next & 0x7fffffffu : ~next;
-                    const float both =
-                        __builtin_bit_cast(float, b) + __builtin_bit_cast(float, c);
-                    best = best == 0xffffffffu ? best : key_of(both);
-                }
-                my_stands[g] = best;
+                // A NaN's key stays above all.
+                if (a.bias && next > kNone && best != 0x7fffffff)
+                    best = key_of(float_of(best) + float_of(next));
+                stands[g] = best;
             }
             wave_fence();
             int g = e0 / per, left = per - (e0 - g * per);
-            bool keep = g < a.groups && in_best(my_stands, a.groups, g, a.kept);
+            bool keep = g < a.groups && in_best(stands, a.groups, g, a.kept);
 #pragma unroll
             for (int j = 0; j < Q; ++j) {
                 if (left == 0) {
                     ++g;
                     left = per;
-                    keep = g < a.groups && in_best(my_stands, a.groups, g, a.kept);
+                    keep = g < a.groups && in_best(stands, a.groups, g, a.kept);
                 }
-                if (!keep) key[j] = 0;
+                if (!keep) key[j] = kGone;
                 --left;
             }
         }
         for (int i = 0; i < a.k; ++i) {
-            unsigned best = 0;
+            int best = key[0];
 #pragma unroll
-            for (int j = 0; j < Q; ++j) best = key[j] > best ? key[j] : best;
-            const unsigned most = lanes_max_key(best, W);
-            const unsigned long long has = __ballot(best == most) & mine;
-            if (lane == 0 && most == 0) {
-                at[i] = -1;
-                ps[i] = 0.0f;
-            }
-            if (most && (t & 63) == __ffsll(has) - 1) {
-                bool found = false;
+            for (int j = 1; j < Q; ++j) best = key[j] > best ? key[j] : best;
+            best = lanes_max_int(best, W);
+            // The lowest index of that key; then it is gone.
+            int expert = 0x7fffffff;
 #pragma unroll
-                for (int j = 0; j < Q; ++j)
-                    if (!found && key[j] == most) {
-                        found = true;
-                        key[j] = 0;
-                        at[i] = e0 + j;
-                        // Renormalised softmax weights need no row sum: they
-                        // are formed from the chosen logits, below.
-                        ps[i] = a.score == TB_HIP_SCORE_SOFTMAX && a.renorm ? x[j] : s[j];
-                    }
-            }
+            for (int j = Q - 1; j >= 0; --j) expert = key[j] == best ? e0 + j : expert;
+            expert = lanes_min_int(expert, W);
+#pragma unroll
+            for (int j = 0; j < Q; ++j) key[j] = expert == e0 + j ? kGone : key[j];
+            if (lane == 0) at[i] = best > kNone ? expert : -1;
         }
         wave_fence();
-        if (token < a.tokens) {
-            const bool from_logits = a.score == TB_HIP_SCORE_SOFTMAX && a.renorm;
-            float total = 0.0f, most = -__builtin_inff();
+        // The weights of the picks, from their logits again.  Renormalised
+        // softmax weights need only the picks': relative to the first one's
+        // largest no sum is 0.
+        float total = 0.0f, most = -__builtin_inff();
+        const bool among = soft && a.renorm;
+        if (live) {
+            if (among)
+                for (int i = lane; i < a.k; i += W)
+                    if (at[i] >= 0) most = fmaxf(most, element<T>(row, at[i]));
+            if (among) most = lanes_max(most, W);
             if (a.renorm) {
-                if (from_logits)
-                    for (int i = 0; i < a.k; ++i)
-                        if (at[i] >= 0) most = fmaxf(most, ps[i]);
-                for (int i = 0; i < a.k; ++i)
-                    if (at[i] >= 0) total += from_logits ? exp_of<true>(ps[i] - most) : ps[i];
-            }
-            for (int i = lane; i < a.k; i += W) {
-                float w = 0.0f;
-                if (at[i] >= 0) {
-                    w = from_logits ? exp_of<true>(ps[i] - most) : ps[i];
-                    if (a.renorm) w = total == 0.0f ? 0.0f : w / total;
-                }
-                a.experts[token * a.k + i] = at[i];
-                a.weights[token * a.k + i] = w * a.scale;
+                for (int i = lane; i < a.k; i += W)
+                    if (at[i] >= 0) {
+                        const float v = element<T>(row, at[i]);
+                        total += soft ? exp_of<true>(v - most) : sigmoid_of<true>(v);
+                    }
+                total = lanes_sum(total, W);
+                // A NaN logit makes the row's scores NaN, picked or not.
+                if (soft && a.bias) total += inverse - inverse;
             }
         }
+        if (token < a.tokens)
+            for (int i = lane; i < a.k; i += W) {
+                const int expert = at[i];
+                float w = 0.0f;
+                if (expert >= 0) {
+                    const float v = element<T>(row, expert);
+                    w = !soft ? sigmoid_of<true>(v)
+                              : among ? exp_of<true>(v - most) : exp_of<true>(v - top) * inverse;
+                    if (a.renorm) w = total == 0.0f ? 0.0f : w / total;
+                }
+                a.experts[token * a.k + i] = expert;
+                a.weights[token * a.k + i] = w * a.scale;
+            }
         wave_fence();
     }
 }
@@ -288,7 +326,7 @@ __global__ __launch_bounds__(kThreads) void route_backward_kernel(RouteArgs a) {
                         d[j] += at[i] == e0 + j ? a.scale * dw[i] : 0.0f;
             float x[Q];
             if (used)
-                load_row<T, Q>(row, e0, a.n, x);
+                load_row<T, Q>(row, e0, a.n, a.vector, x);
             else
 #pragma unroll
                 for (int j = 0; j < Q; ++j) x[j] = 0.0f;
@@ -331,10 +369,12 @@ __global__ __launch_bounds__(kThreads) void route_backward_kernel(RouteArgs a) {
 // cut into segments, one to a wave: (1) every segment's count of each expert,
 // (2) for each expert the running sum over the segments, (3) the segments
 // again, each choice to its expert's start plus its running sum plus its rank
-// in the segment.  Choices outside the experts count as expert n.
+// in the segment.  Choices outside the experts count as expert n.  Up to
+// kSmallChoices one workgroup does all three.
 
-constexpr int kOrderWaves = 4;
-constexpr size_t kSegment = 512, kMaxSegments = 4096;
+constexpr int kOrderWaves = 4, kSmallWaves = 16;
+constexpr int kBatch = 8;  // choices of a lane on their way at once
+constexpr size_t kSegment = 64 * kBatch, kMaxSegments = 4096, kSmallChoices = 8192;
 
 struct OrderArgs {
     const int *experts;
@@ -345,12 +385,81 @@ struct OrderArgs {
     int *totals;  // [n + 1]
     size_t choices, segment;
     unsigned segments;
-    int n, k;
+    int n, k, bits;
 };
 
-__device__ __forceinline__ int expert_of(const OrderArgs &a, size_t c) {
-    const int e = a.experts[c];
-    return (unsigned)e < (unsigned)a.n ? e : a.n;
+// The experts of choices c0 + lane, + 64, ...; n past c1.
+__device__ __forceinline__ void load_choices(const OrderArgs &a, size_t c0, size_t c1,
+                                             int (&e)[kBatch]) {
+    const size_t c = c0 + (threadIdx.x & 63);
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) e[j] = c + 64 * j < c1 ? a.experts[c + 64 * j] : a.n;
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) e[j] = (unsigned)e[j] < (unsigned)a.n ? e[j] : a.n;
+}
+
+// Adds a wave's segment to its counts in LDS.
+__device__ __forceinline__ void count_segment(const OrderArgs &a, size_t c0, size_t c1,
+                                              int *count) {
+    const int lane = threadIdx.x & 63;
+    for (size_t c = c0; c < c1; c += kSegment) {
+        int e[kBatch];
+        load_choices(a, c, c1, e);
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j)
+            if (c + lane + 64 * j < c1) atomicAdd(&count[e[j]], 1);
+    }
+}
+
+// Writes a wave's segment; next[e] is the row of its next choice of expert e.
+__device__ __forceinline__ void place_segment(const OrderArgs &a, size_t c0, size_t c1,
+                                              int *next) {
+    const int lane = threadIdx.x & 63;
+    for (size_t cb = c0; cb < c1; cb += kSegment) {
+        int e[kBatch], row[kBatch];
+        load_choices(a, cb, c1, e);
+        float w[kBatch];
+        if (a.weights)
+#pragma unroll
+            for (int j = 0; j < kBatch; ++j)
+                w[j] = cb + lane + 64 * j < c1 ? a.weights[cb + lane + 64 * j] : 0.0f;
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) {
+            const bool live = cb + lane + 64 * j < c1;
+            // The lanes with the same expert.
+            unsigned long long same = __ballot(live);
+            for (int b = 0; b < a.bits; ++b) {
+                const bool set = (e[j] >> b) & 1;
+                const unsigned long long all = __ballot(set);
+                same &= set ? all : ~all;
+            }
+            const int rank = __popcll(same & ((1ull << lane) - 1));
+            row[j] = live ? next[e[j]] + rank : 0;
+            wave_fence();
+            if (live && rank == 0) next[e[j]] = row[j] + __popcll(same);
+            wave_fence();
+        }
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) {
+            const size_t c = cb + lane + 64 * j;
+            if (c < c1) {
+                const bool known = e[j] < a.n;
+                a.tokens[row[j]] = known ? (int)((unsigned)c / (unsigned)a.k) : -1;
+                a.positions[c] = known ? row[j] : -1;
+                if (a.weights) a.row_weights[row[j]] = known ? w[j] : 0.0f;
+            }
+        }
+    }
+}
+
+// Sum over the lanes up to this one.
+__device__ __forceinline__ int running_sum(int v) {
+    const int lane = threadIdx.x & 63;
+    for (int off = 1; off < 64; off *= 2) {
+        const int o = __shfl_up(v, off);
+        if (lane >= off) v += o;
+    }
+    return v;
 }
 
 __global__ __launch_bounds__(kOrderWaves * 64) void order_count_kernel(OrderArgs a) {
@@ -362,8 +471,7 @@ __global__ __launch_bounds__(kOrderWaves * 64) void order_count_kernel(OrderArgs
     for (int e = lane; e <= a.n; e += 64) count[e] = 0;
     wave_fence();
     const size_t c0 = seg * a.segment;
-    const size_t c1 = c0 + a.segment < a.choices ? c0 + a.segment : a.choices;
-    for (size_t c = c0 + lane; c < c1; c += 64) atomicAdd(&count[expert_of(a, c)], 1);
+    count_segment(a, c0, c0 + a.segment < a.choices ? c0 + a.segment : a.choices, count);
     wave_fence();
     for (int e = lane; e <= a.n; e += 64) a.counts[(size_t)e * a.segments + seg] = count[e];
 }
@@ -376,12 +484,7 @@ __global__ __launch_bounds__(256) void order_sum_kernel(OrderArgs a) {
     int before = 0;
     for (unsigned s0 = 0; s0 < a.segments; s0 += 256) {
         const unsigned s = s0 + t;
-        const int v = s < a.segments ? row[s] : 0;
-        int sum = v;
-        for (int off = 1; off < 64; off *= 2) {
-            const int o = __shfl_up(sum, off);
-            if (lane >= off) sum += o;
-        }
+        const int v = s < a.segments ? row[s] : 0, sum = running_sum(v);
         if (lane == 63) wave_total[t >> 6] = sum;
         __syncthreads();
         int below = 0, all = 0;
@@ -396,59 +499,66 @@ __global__ __launch_bounds__(256) void order_sum_kernel(OrderArgs a) {
     if (t == 0) a.totals[blockIdx.x] = before;
 }
 
+// Every expert's start from the totals, by one wave.
+__device__ __forceinline__ void find_starts(const OrderArgs &a, const int *totals, int *start,
+                                            bool write) {
+    const int lane = threadIdx.x & 63;
+    int before = 0;
+    for (int e0 = 0; e0 <= a.n; e0 += 64) {
+        const int e = e0 + lane, v = e <= a.n ? totals[e] : 0, sum = running_sum(v);
+        if (e <= a.n) {
+            start[e] = before + sum - v;
+            if (write) a.offsets[e] = before + sum - v;
+        }
+        before += __builtin_amdgcn_readlane(sum, 63);
+    }
+}
+
 __global__ __launch_bounds__(kOrderWaves * 64) void order_place_kernel(OrderArgs a) {
     extern __shared__ int lds[];
     const int t = threadIdx.x, wave = t >> 6, lane = t & 63;
     int *start = lds, *next = lds + (a.n + 1) * (1 + wave);
-    // Every expert's start: wave 0 runs along the totals.
-    if (wave == 0) {
-        int before = 0;
-        for (int e0 = 0; e0 <= a.n; e0 += 64) {
-            const int e = e0 + lane, v = e <= a.n ? a.totals[e] : 0;
-            int sum = v;
-            for (int off = 1; off < 64; off *= 2) {
-                const int o = __shfl_up(sum, off);
-                if (lane >= off) sum += o;
-            }
-            if (e <= a.n) {
-                start[e] = before + sum - v;
-                if (blockIdx.x == 0) a.offsets[e] = before + sum - v;
-            }
-            before += __shfl(sum, 63);
-        }
-    }
+    if (wave == 0) find_starts(a, a.totals, start, blockIdx.x == 0);
     __syncthreads();
     const unsigned seg = blockIdx.x * kOrderWaves + wave;
     if (seg >= a.segments) return;
     for (int e = lane; e <= a.n; e += 64)
         next[e] = start[e] + a.counts[(size_t)e * a.segments + seg];
     wave_fence();
-    int bits = 1;
-    while ((1 << bits) <= a.n) ++bits;
     const size_t c0 = seg * a.segment;
+    place_segment(a, c0, c0 + a.segment < a.choices ? c0 + a.segment : a.choices, next);
+}
+
+// All of it in one workgroup: LDS holds the totals and each wave's counts.
+__global__ __launch_bounds__(kSmallWaves * 64) void order_small_kernel(OrderArgs a) {
+    extern __shared__ int lds[];
+    const int t = threadIdx.x, wave = t >> 6, columns = a.n + 1;
+    int *start = lds, *next = lds + columns * (1 + wave);
+    for (int i = t; i < columns * (1 + kSmallWaves); i += kSmallWaves * 64) lds[i] = 0;
+    __syncthreads();
+    const size_t c0 = wave * a.segment < a.choices ? wave * a.segment : a.choices;
     const size_t c1 = c0 + a.segment < a.choices ? c0 + a.segment : a.choices;
-    for (size_t i = c0; i < c1; i += 64) {
-        const size_t c = i + lane;
-        const bool live = c < c1;
-        const int e = live ? expert_of(a, c) : 0;
-        // The lanes with the same expert.
-        unsigned long long same = __ballot(live);
-        for (int b = 0; b < bits; ++b) {
-            const unsigned long long set = __ballot((e >> b) & 1);
-            same &= (e >> b) & 1 ? set : ~set;
+    count_segment(a, c0, c1, next);
+    __syncthreads();
+    // Counts to running sums over the waves; the totals behind.
+    for (int e = t; e < columns; e += kSmallWaves * 64) {
+        int before = 0;
+        for (int w = 0; w < kSmallWaves; ++w) {
+            const int v = lds[columns * (1 + w) + e];
+            lds[columns * (1 + w) + e] = before;
+            before += v;
         }
-        const int rank = __popcll(same & ((1ull << lane) - 1));
-        const int row = live ? next[e] + rank : 0;
-        wave_fence();
-        if (live && rank == 0) next[e] = row + __popcll(same);
-        wave_fence();
-        if (live) {
-            const bool known = e < a.n;
-            a.tokens[row] = known ? (int)(c / (unsigned)a.k) : -1;
-            a.positions[c] = known ? row : -1;
-            if (a.weights) a.row_weights[row] = known ? a.weights[c] : 0.0f;
-        }
+        start[e] = before;
     }
+    __syncthreads();
+    if (wave == 0) find_starts(a, start, start, true);
+    __syncthreads();
+    for (int i = t; i < columns * kSmallWaves; i += kSmallWaves * 64) {
+        const int e = i % columns;
+        lds[columns + i] += start[e];
+    }
+    __syncthreads();
+    place_segment(a, c0, c1, next);
 }
 
 // --------------------------------------------------------------------------
@@ -477,26 +587,33 @@ unsigned grid_for(const RouteArgs &a) {
 }
 
 // 8 experts a lane up to 512 experts, 16 above, where 64 lanes need them.
-template <class T>
+template <class T, int Q>
 void launch_route(RouteArgs &a, hipStream_t q) {
-    if (a.n <= 512) {
-        a.lanes = lanes_for(a.n, 8);
-        route_kernel<T, 8><<<grid_for(a), kThreads, 0, q>>>(a);
-    } else {
-        a.lanes = 64;
-        route_kernel<T, 16><<<grid_for(a), kThreads, 0, q>>>(a);
-    }
+    a.lanes = lanes_for(a.n, Q);
+    const size_t words = route_words(a.lanes * Q, a.k, a.kept < a.groups);
+    route_kernel<T, Q><<<grid_for(a), kThreads, kThreads / a.lanes * words * sizeof(int), q>>>(a);
 }
 
-template <class T>
+template <class T, int Q>
 void launch_backward(RouteArgs &a, hipStream_t q) {
-    if (a.n <= 512) {
-        a.lanes = lanes_for(a.n, 8);
-        route_backward_kernel<T, 8><<<grid_for(a), kThreads, 0, q>>>(a);
-    } else {
-        a.lanes = 64;
-        route_backward_kernel<T, 16><<<grid_for(a), kThreads, 0, q>>>(a);
-    }
+    a.lanes = lanes_for(a.n, Q);
+    route_backward_kernel<T, Q><<<grid_for(a), kThreads, 0, q>>>(a);
+}
+
+// Rows that start on 16 bytes and hold whole lanes' experts.
+int vector_rows(const void *p, size_t stride, int n) {
+    return multiple_of(p, 16) && stride % 16 == 0 && n % (n <= 512 ? 8 : 16) == 0;
+}
+
+// Calls f with a zero of the type.
+template <class F>
+void with_type(int dtype, F f) {
+    if (dtype == TB_HIP_F32)
+        f(0.0f);
+    else if (dtype == TB_HIP_BF16)
+        f((__bf16)0.0f);
+    else
+        f((_Float16)0.0f);
 }
 
 struct OrderShape {
@@ -546,12 +663,13 @@ extern "C" int tb_hip_route_device(const void *logits, size_t row_stride, const 
     a.scale = scale;
     hipStream_t q = reinterpret_cast<hipStream_t>(stream);
     (void)hipGetLastError();
-    if (dtype == TB_HIP_F32)
-        launch_route<float>(a, q);
-    else if (dtype == TB_HIP_BF16)
-        launch_route<__bf16>(a, q);
-    else
-        launch_route<_Float16>(a, q);
+    a.vector = vector_rows(logits, row_stride, n_experts);
+    with_type(dtype, [&](auto zero) {
+        if (n_experts <= 512)
+            launch_route<decltype(zero), 8>(a, q);
+        else
+            launch_route<decltype(zero), 16>(a, q);
+    });
     return hipGetLastError() == hipSuccess;
 }
 
@@ -577,12 +695,13 @@ extern "C" int tb_hip_route_backward_device(const void *logits, size_t row_strid
     a.scale = scale;
     hipStream_t q = reinterpret_cast<hipStream_t>(stream);
     (void)hipGetLastError();
-    if (dtype == TB_HIP_F32)
-        launch_backward<float>(a, q);
-    else if (dtype == TB_HIP_BF16)
-        launch_backward<__bf16>(a, q);
-    else
-        launch_backward<_Float16>(a, q);
+    a.vector = vector_rows(logits, row_stride, n_experts);
+    with_type(dtype, [&](auto zero) {
+        if (n_experts <= 512)
+            launch_backward<decltype(zero), 8>(a, q);
+        else
+            launch_backward<decltype(zero), 16>(a, q);
+    });
     return hipGetLastError() == hipSuccess;
 }
 
@@ -615,10 +734,16 @@ extern "C" int tb_hip_expert_order_device(const int *experts, const float *weigh
     a.segments = s.segments;
     a.n = n_experts;
     a.k = k;
+    while ((1 << a.bits) <= n_experts) ++a.bits;
     hipStream_t q = reinterpret_cast<hipStream_t>(stream);
-    const unsigned blocks = (s.segments + kOrderWaves - 1) / kOrderWaves;
     const size_t row = (n_experts + 1) * sizeof(int);
     (void)hipGetLastError();
+    if (a.choices <= kSmallChoices && row * (1 + kSmallWaves) <= 64 * 1024) {
+        a.segment = (a.choices + kSmallWaves * 64 - 1) / (kSmallWaves * 64) * 64;
+        order_small_kernel<<<1, kSmallWaves * 64, row * (1 + kSmallWaves), q>>>(a);
+        return hipGetLastError() == hipSuccess;
+    }
+    const unsigned blocks = (s.segments + kOrderWaves - 1) / kOrderWaves;
     order_count_kernel<<<blocks, kOrderWaves * 64, kOrderWaves * row, q>>>(a);
     order_sum_kernel<<<n_experts + 1, 256, 0, q>>>(a);
     order_place_kernel<<<blocks, kOrderWaves * 64, (1 + kOrderWaves) * row, q>>>(a);
