@@ -38,6 +38,7 @@ struct RouteArgs {
     char *dlogits;
     size_t tokens;
     int n, k, groups, kept, lanes, score, renorm, vector;
+    int log_per;  // of a group's experts, -1 if they are no power of two
     float scale;
 };
 
@@ -123,30 +124,89 @@ __device__ __forceinline__ void load_row(const char *row, int e0, int n, int vec
 }
 
 // Whether all[i] is among the `kept` highest of all[count], ties to the lower
-// index.
+// index.  Keys above kGone.
 __device__ __forceinline__ bool in_best(const int *all, int count, int i, int kept) {
     const int v = all[i];
     int before = 0;
-    for (int j = 0; j < count; ++j) before += all[j] > v || (all[j] == v && j < i);
+    for (int j0 = 0; j0 < count; j0 += 8) {
+        int other[8];  // read at once
+#pragma unroll
+        for (int j = 0; j < 8; ++j) other[j] = j0 + j < count ? all[j0 + j] : kGone;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) before += other[j] > (j0 + j < i ? v - 1 : v);
+    }
     return before < kept;
 }
 
-// LDS of a token: its picks, with groups also the keys and the groups'
-// standings, one word apart from the next token's so that tokens lie in
-// different banks.
-__host__ __device__ inline int route_words(int span, int k, bool groups) {
-    return (k + (groups ? 2 * span : 0)) | 1;
+// The two best keys of a set.
+struct Two {
+    int best, next;
+};
+__device__ __forceinline__ Two joined(Two a, Two b) {
+    const int low = a.best < b.best ? a.best : b.best, next = a.next > b.next ? a.next : b.next;
+    return {a.best > b.best ? a.best : b.best, low > next ? low : next};
+}
+// A group's: the best key, with a bias the sum of the two best that can be
+// chosen.  A NaN's key stays above all.
+__device__ __forceinline__ int standing(Two t, const float *bias) {
+    int v = t.best;
+    if (bias && t.next > kNone && v != 0x7fffffff) v = key_of(float_of(v) + float_of(t.next));
+    return v > kGone ? v : kGone + 1;
 }
 
-template <class T, int Q>
+// The keys of the kept groups, groups of 2^log_per experts: the two best of
+// each in registers and between lanes, the standings through LDS.
+template <int Q>
+__device__ __forceinline__ void keep_groups(const RouteArgs &a, int e0, int lane, int *stands,
+                                            int (&key)[Q]) {
+    Two two[Q];
+#pragma unroll
+    for (int j = 0; j < Q; ++j) two[j] = {key[j], kGone};
+    // Leaders: the first of every group, or of the lane.
+#pragma unroll
+    for (int l = 0; (1 << l) < Q; ++l)
+        if (a.log_per > l) {
+#pragma unroll
+            for (int j = 0; j < Q; j += 2 << l) two[j] = joined(two[j], two[j + (1 << l)]);
+        }
+    constexpr int kLogQ = Q == 8 ? 3 : 4;
+    const int share = a.log_per > kLogQ ? 1 << (a.log_per - kLogQ) : 1;  // lanes of a group
+    for (int off = 1; off < share; off *= 2)
+        two[0] = joined(two[0], Two{__shfl_xor(two[0].best, off), __shfl_xor(two[0].next, off)});
+    const int seg = a.log_per < kLogQ ? (1 << a.log_per) - 1 : Q - 1;
+#pragma unroll
+    for (int j = 0; j < Q; ++j)
+        if ((j & seg) == 0 && e0 + j < a.n && (lane & (share - 1)) == 0)
+            stands[(e0 + j) >> a.log_per] = standing(two[j], a.bias);
+    wave_fence();
+    bool keep = false;
+#pragma unroll
+    for (int j = 0; j < Q; ++j) {
+        if ((j & seg) == 0)
+            keep = e0 + j < a.n && in_best(stands, a.groups, (e0 + j) >> a.log_per, a.kept);
+        if (!keep) key[j] = kGone;
+    }
+}
+
+// LDS of a token: its picks and their scores, with groups also the keys and
+// the groups' standings, one word apart from the next token's so that tokens lie in
+// different banks.
+__host__ __device__ inline int route_words(int span, int k, int groups) {
+    return (2 * k + (groups ? 2 * span : 0)) | 1;
+}
+
+// How groups are kept: not at all, of a power of two of experts, of others.
+enum { kAll, kEven, kUneven };
+
+template <class T, int Q, int GROUPS>
 __global__ __launch_bounds__(kThreads) void route_kernel(RouteArgs a) {
     extern __shared__ int lds[];
     const int W = a.lanes, per_block = kThreads / W, t = threadIdx.x;
     const int lane = t & (W - 1), slot = t / W;
     const int e0 = lane * Q, span = W * Q;
-    const bool grouped = a.kept < a.groups;
-    int *at = lds + slot * route_words(span, a.k, grouped), *keys = at + a.k,
+    int *at = lds + slot * route_words(span, a.k, GROUPS), *keys = at + 2 * a.k,
         *stands = keys + span;
+    float *scores = reinterpret_cast<float *>(at + a.k);
     const bool soft = a.score == TB_HIP_SCORE_SOFTMAX;
     for (size_t base = (size_t)blockIdx.x * per_block; base < a.tokens;
          base += (size_t)gridDim.x * per_block) {
@@ -171,31 +231,27 @@ __global__ __launch_bounds__(kThreads) void route_kernel(RouteArgs a) {
             for (int j = 0; j < Q; ++j) sum += e0 + j < a.n ? exp_of<true>(x[j] - top) : 0.0f;
             inverse = 1.0f / lanes_sum(sum, W);
         }
-#pragma unroll
-        for (int j = 0; j < Q; ++j) key[j] = key_of(x[j]);
         if (a.bias) {
 #pragma unroll
             for (int j = 0; j < Q; ++j) {
+                const float b = e0 + j < a.n ? a.bias[e0 + j] : 0.0f;
                 const float s = soft ? exp_of<true>(x[j] - top) * inverse : sigmoid_of<true>(x[j]);
-                if (key[j] > kNone) key[j] = key_of(s + a.bias[e0 + j]);
+                key[j] = x[j] == -__builtin_inff() ? kGone : key_of(s + b);
             }
+        } else {
+#pragma unroll
+            for (int j = 0; j < Q; ++j) key[j] = key_of(x[j]);
         }
-        if (grouped) {
+        if constexpr (GROUPS == kEven) keep_groups<Q>(a, e0, lane, stands, key);
+        if constexpr (GROUPS == kUneven) {
             const int per = a.n / a.groups;
 #pragma unroll
             for (int j = 0; j < Q; ++j) keys[e0 + j] = key[j];
             wave_fence();
             for (int g = lane; g < a.groups; g += W) {
-                int best = kGone, next = kGone;
-                for (int i = 0; i < per; ++i) {
-                    const int v = keys[g * per + i], low = v < best ? v : best;
-                    next = low > next ? low : next;
-                    best = v > best ? v : best;
-                }
-                // A NaN's key stays above all.
-                if (a.bias && next > kNone && best != 0x7fffffff)
-                    best = key_of(float_of(best) + float_of(next));
-                stands[g] = best;
+                Two two = {kGone, kGone};
+                for (int i = 0; i < per; ++i) two = joined(two, Two{keys[g * per + i], kGone});
+                stands[g] = standing(two, a.bias);
             }
             wave_fence();
             int g = e0 / per, left = per - (e0 - g * per);
@@ -227,49 +283,57 @@ __global__ __launch_bounds__(kThreads) void route_kernel(RouteArgs a) {
         }
         wave_fence();
         // The weights of the picks, from their logits again.  Renormalised
-        // softmax weights need only the picks': relative to the first one's
-        // largest no sum is 0.
-        float total = 0.0f, most = -__builtin_inff();
+        // softmax weights need only the picks': relative to the largest of
+        // them no sum is 0.
         const bool among = soft && a.renorm;
-        if (live) {
-            if (among)
-                for (int i = lane; i < a.k; i += W)
-                    if (at[i] >= 0) most = fmaxf(most, element<T>(row, at[i]));
-            if (among) most = lanes_max(most, W);
-            if (a.renorm) {
-                for (int i = lane; i < a.k; i += W)
-                    if (at[i] >= 0) {
-                        const float v = element<T>(row, at[i]);
-                        total += soft ? exp_of<true>(v - most) : sigmoid_of<true>(v);
-                    }
-                total = lanes_sum(total, W);
-                // A NaN logit makes the row's scores NaN, picked or not.
-                if (soft && a.bias) total += inverse - inverse;
+        float total = 0.0f;
+        if (among) {
+            top = -__builtin_inff();
+            for (int i = lane; i < a.k; i += W)
+                if (at[i] >= 0) top = fmaxf(top, element<T>(row, at[i]));
+            top = lanes_max(top, W);
+        }
+        for (int i = lane; i < a.k; i += W) {
+            float s = 0.0f;
+            if (at[i] >= 0) {
+                const float v = element<T>(row, at[i]);
+                s = soft ? exp_of<true>(v - top) : sigmoid_of<true>(v);
             }
+            scores[i] = s;
+            total += s;
+        }
+        float factor = a.scale;
+        if (a.renorm) {
+            total = lanes_sum(total, W);
+            // A NaN logit makes the row's scores NaN, picked or not.
+            if (soft && a.bias) total += inverse - inverse;
+        } else {
+            factor *= inverse;
         }
         if (token < a.tokens)
             for (int i = lane; i < a.k; i += W) {
-                const int expert = at[i];
-                float w = 0.0f;
-                if (expert >= 0) {
-                    const float v = element<T>(row, expert);
-                    w = !soft ? sigmoid_of<true>(v)
-                              : among ? exp_of<true>(v - most) : exp_of<true>(v - top) * inverse;
-                    if (a.renorm) w = total == 0.0f ? 0.0f : w / total;
-                }
-                a.experts[token * a.k + i] = expert;
-                a.weights[token * a.k + i] = w * a.scale;
+                float w = scores[i];
+                if (a.renorm) w = total == 0.0f ? 0.0f : w / total;
+                // No pick has weight 0 also where the row is NaN.
+                a.experts[token * a.k + i] = at[i];
+                a.weights[token * a.k + i] = at[i] >= 0 ? w * factor : 0.0f;
             }
         wave_fence();
     }
 }
 
+// A lane forms what belongs to its picks and puts it into the token's row in
+// LDS, from which every lane takes its experts'.  Only softmax scores that are
+// not renormalised need the whole row of logits.
 template <class T, int Q>
 __global__ __launch_bounds__(kThreads) void route_backward_kernel(RouteArgs a) {
+    __shared__ __attribute__((aligned(16))) float rows[kThreads * Q];
+    typedef float floats __attribute__((ext_vector_type(4)));
     const int W = a.lanes, per_block = kThreads / W, t = threadIdx.x;
-    const int lane = t & (W - 1), slot = t / W;
-    const int e0 = lane * Q;
-    const bool soft = a.score == TB_HIP_SCORE_SOFTMAX;
+    const int lane = t & (W - 1), slot = t / W, e0 = lane * Q;
+    const bool soft = a.score == TB_HIP_SCORE_SOFTMAX, whole = soft && !a.renorm;
+    float *d = rows + slot * W * Q;
+    floats *mine = reinterpret_cast<floats *>(d + e0);
     for (size_t base = (size_t)blockIdx.x * per_block; base < a.tokens;
          base += (size_t)gridDim.x * per_block) {
         const size_t token = base + slot;
@@ -277,90 +341,108 @@ __global__ __launch_bounds__(kThreads) void route_backward_kernel(RouteArgs a) {
         const char *row = a.logits + token * a.stride;
         const int *at = a.chosen + token * a.k;
         const float *dw = a.dweights + token * a.k;
-        float d[Q];
 #pragma unroll
-        for (int j = 0; j < Q; ++j) d[j] = 0.0f;
+        for (int j = 0; j < Q / 4; ++j) mine[j] = (floats){0, 0, 0, 0};
+        wave_fence();
         int used = 0;
+        float top = -__builtin_inff();
         if (live)
-            for (int i = 0; i < a.k; ++i) used += (unsigned)at[i] < (unsigned)a.n;
+            for (int i = lane; i < a.k; i += W)
+                if ((unsigned)at[i] < (unsigned)a.n) {
+                    used = 1;
+                    if (soft && a.renorm) top = fmaxf(top, element<T>(row, at[i]));
+                }
+        used = lanes_max_int(used, W);
         if (a.renorm) {
-            // w' of the chosen from their logits alone, as quotients: a single
-            // choice has w' = 1 and no gradient, exactly.
-            float most = -__builtin_inff(), total = 0.0f, dot = 0.0f;
-            if (used) {
-                if (soft)
-                    for (int i = 0; i < a.k; ++i)
-                        if ((unsigned)at[i] < (unsigned)a.n)
-                            most = fmaxf(most, element<T>(row, at[i]));
-                for (int i = 0; i < a.k; ++i)
+            // w' of the picks, as quotients: a single one has w' = 1 and no
+            // gradient, exactly.
+            if (soft) top = lanes_max(top, W);
+            float total = 0.0f, dot = 0.0f;
+            if (live)
+                for (int i = lane; i < a.k; i += W)
                     if ((unsigned)at[i] < (unsigned)a.n) {
                         const float x = element<T>(row, at[i]);
-                        total += soft ? exp_of<true>(x - most) : sigmoid_of<true>(x);
+                        const float s = soft ? exp_of<true>(x - top) : sigmoid_of<true>(x);
+                        d[at[i]] = s;
+                        total += s;
                     }
-                // A sum of 0 gave weights of 0.
-                if (total == 0.0f) used = 0;
-            }
-            if (used) {
-                for (int i = 0; i < a.k; ++i)
+            total = lanes_sum(total, W);
+            wave_fence();
+            if (live)
+                for (int i = lane; i < a.k; i += W)
+                    if ((unsigned)at[i] < (unsigned)a.n)
+                        dot += d[at[i]] / total * (a.scale * dw[i]);
+            dot = lanes_sum(dot, W);
+            if (live)
+                for (int i = lane; i < a.k; i += W)
                     if ((unsigned)at[i] < (unsigned)a.n) {
-                        const float x = element<T>(row, at[i]);
-                        const float s = soft ? exp_of<true>(x - most) : sigmoid_of<true>(x);
-                        dot += s / total * (a.scale * dw[i]);
+                        // 1 - s as the sigmoid of -x, without cancelling.  A sum
+                        // of 0 gave weights of 0.
+                        const float rest =
+                            soft ? 1.0f : sigmoid_of<true>(-element<T>(row, at[i]));
+                        const float w = d[at[i]] / total;
+                        d[at[i]] = total == 0.0f ? 0.0f : w * rest * (a.scale * dw[i] - dot);
                     }
-                for (int i = 0; i < a.k; ++i)
-                    if (at[i] >= e0 && at[i] < e0 + Q && at[i] < a.n) {
+        } else if (live) {
+            for (int i = lane; i < a.k; i += W)
+                if ((unsigned)at[i] < (unsigned)a.n) {
+                    float g = a.scale * dw[i];
+                    if (!soft) {
                         const float x = element<T>(row, at[i]);
-                        const float s = soft ? exp_of<true>(x - most) : sigmoid_of<true>(x);
-                        // 1 - s as the sigmoid of -x, without cancelling.
-                        const float rest = soft ? 1.0f : sigmoid_of<true>(-x);
-                        const float v = s / total * rest * (a.scale * dw[i] - dot);
-#pragma unroll
-                        for (int j = 0; j < Q; ++j) d[j] += at[i] == e0 + j ? v : 0.0f;
+                        g *= sigmoid_of<true>(x) * sigmoid_of<true>(-x);
                     }
-            }
-        } else {
-            if (used)
-                for (int i = 0; i < a.k; ++i)
+                    d[at[i]] = g;
+                }
+        }
+        wave_fence();
+        float v[Q];
 #pragma unroll
-                    for (int j = 0; j < Q; ++j)
-                        d[j] += at[i] == e0 + j ? a.scale * dw[i] : 0.0f;
+        for (int j = 0; j < Q; ++j) v[j] = mine[j / 4][j % 4];
+        if (whole) {
             float x[Q];
             if (used)
                 load_row<T, Q>(row, e0, a.n, a.vector, x);
             else
 #pragma unroll
                 for (int j = 0; j < Q; ++j) x[j] = 0.0f;
-            if (soft) {
-                float top = -__builtin_inff(), sum = 0.0f, dot = 0.0f;
+            float sum = 0.0f, dot = 0.0f;
 #pragma unroll
-                for (int j = 0; j < Q; ++j) top = fmaxf(top, x[j]);
-                top = lanes_max(top, W);
+            for (int j = 0; j < Q; ++j) top = fmaxf(top, x[j]);
+            top = lanes_max(top, W);
 #pragma unroll
-                for (int j = 0; j < Q; ++j) {
-                    x[j] = e0 + j < a.n ? exp_of<true>(x[j] - top) : 0.0f;
-                    sum += x[j];
-                }
-                const float inverse = 1.0f / lanes_sum(sum, W);
+            for (int j = 0; j < Q; ++j) {
+                x[j] = e0 + j < a.n ? exp_of<true>(x[j] - top) : 0.0f;
+                sum += x[j];
+            }
+            const float inverse = 1.0f / lanes_sum(sum, W);
 #pragma unroll
-                for (int j = 0; j < Q; ++j) {
-                    x[j] *= inverse;
-                    dot += d[j] * x[j];
-                }
-                dot = lanes_sum(dot, W);
+            for (int j = 0; j < Q; ++j) {
+                x[j] *= inverse;
+                dot += v[j] * x[j];
+            }
+            dot = lanes_sum(dot, W);
 #pragma unroll
-                for (int j = 0; j < Q; ++j) d[j] = used ? x[j] * (d[j] - dot) : 0.0f;
+            for (int j = 0; j < Q; ++j) v[j] = used ? x[j] * (v[j] - dot) : 0.0f;
+        }
+        if (live) {
+            T *out = reinterpret_cast<T *>(a.dlogits) + token * a.n + e0;
+            if (a.vector) {
+                typedef Vec<T, 16> X;
+                if (e0 < a.n)
+#pragma unroll
+                    for (int p = 0; p < Q / X::n; ++p) {
+                        float part[X::n];
+#pragma unroll
+                        for (int j = 0; j < X::n; ++j) part[j] = v[p * X::n + j];
+                        reinterpret_cast<typename X::raw *>(out)[p] = X::pack(part);
+                    }
             } else {
 #pragma unroll
                 for (int j = 0; j < Q; ++j)
-                    if (d[j] != 0.0f) d[j] *= sigmoid_of<true>(x[j]) * sigmoid_of<true>(-x[j]);
+                    if (e0 + j < a.n) out[j] = (T)v[j];
             }
         }
-        if (live) {
-            T *out = reinterpret_cast<T *>(a.dlogits) + token * a.n;
-#pragma unroll
-            for (int j = 0; j < Q; ++j)
-                if (e0 + j < a.n) out[e0 + j] = (T)d[j];
-        }
+        wave_fence();
     }
 }
 
@@ -586,12 +668,18 @@ unsigned grid_for(const RouteArgs &a) {
     return (unsigned)(want < kMaxGrid ? want : kMaxGrid);
 }
 
-// 8 experts a lane up to 512 experts, 16 above, where 64 lanes need them.
-template <class T, int Q>
+// Experts a lane.  Forward 16 above 16 experts, which halves what lanes do for
+// their token (163,840 tokens, us, 8 / 16 a lane: 4 of 64 20.5 / 15.6, 2 of 16
+// 6.8 / 7.0, 8 of 128 of 81,920 tokens 30.0 / 24.3); backward 8, which
+// keeps more loads under way, as long as 64 lanes hold a token's.
+constexpr int kForwardEight = 16, kBackwardEight = 512;
+
+template <class T, int Q, int GROUPS>
 void launch_route(RouteArgs &a, hipStream_t q) {
     a.lanes = lanes_for(a.n, Q);
-    const size_t words = route_words(a.lanes * Q, a.k, a.kept < a.groups);
-    route_kernel<T, Q><<<grid_for(a), kThreads, kThreads / a.lanes * words * sizeof(int), q>>>(a);
+    const size_t words = route_words(a.lanes * Q, a.k, GROUPS);
+    route_kernel<T, Q, GROUPS>
+        <<<grid_for(a), kThreads, kThreads / a.lanes * words * sizeof(int), q>>>(a);
 }
 
 template <class T, int Q>
@@ -601,8 +689,8 @@ void launch_backward(RouteArgs &a, hipStream_t q) {
 }
 
 // Rows that start on 16 bytes and hold whole lanes' experts.
-int vector_rows(const void *p, size_t stride, int n) {
-    return multiple_of(p, 16) && stride % 16 == 0 && n % (n <= 512 ? 8 : 16) == 0;
+int vector_rows(const void *p, size_t stride, int n, int q) {
+    return multiple_of(p, 16) && stride % 16 == 0 && n % q == 0;
 }
 
 // Calls f with a zero of the type.
@@ -658,17 +746,23 @@ extern "C" int tb_hip_route_device(const void *logits, size_t row_stride, const 
     a.k = k;
     a.groups = groups;
     a.kept = groups_kept;
+    const int per = n_experts / groups;
+    a.log_per = per & (per - 1) ? -1 : __builtin_ctz(per);
     a.score = score;
     a.renorm = renormalise != 0;
     a.scale = scale;
     hipStream_t q = reinterpret_cast<hipStream_t>(stream);
     (void)hipGetLastError();
-    a.vector = vector_rows(logits, row_stride, n_experts);
+    const bool eight = n_experts <= kForwardEight;
+    a.vector = vector_rows(logits, row_stride, n_experts, eight ? 8 : 16);
     with_type(dtype, [&](auto zero) {
-        if (n_experts <= 512)
-            launch_route<decltype(zero), 8>(a, q);
+        typedef decltype(zero) T;
+        if (groups_kept == groups)
+            eight ? launch_route<T, 8, kAll>(a, q) : launch_route<T, 16, kAll>(a, q);
+        else if (a.log_per >= 0)
+            eight ? launch_route<T, 8, kEven>(a, q) : launch_route<T, 16, kEven>(a, q);
         else
-            launch_route<decltype(zero), 16>(a, q);
+            eight ? launch_route<T, 8, kUneven>(a, q) : launch_route<T, 16, kUneven>(a, q);
     });
     return hipGetLastError() == hipSuccess;
 }
@@ -695,9 +789,11 @@ extern "C" int tb_hip_route_backward_device(const void *logits, size_t row_strid
     a.scale = scale;
     hipStream_t q = reinterpret_cast<hipStream_t>(stream);
     (void)hipGetLastError();
-    a.vector = vector_rows(logits, row_stride, n_experts);
+    const bool eight = n_experts <= kBackwardEight;
+    a.vector = vector_rows(logits, row_stride, n_experts, eight ? 8 : 16) &&
+               multiple_of(dlogits, 16);
     with_type(dtype, [&](auto zero) {
-        if (n_experts <= 512)
+        if (eight)
             launch_backward<decltype(zero), 8>(a, q);
         else
             launch_backward<decltype(zero), 16>(a, q);
