@@ -37,7 +37,7 @@ struct RouteArgs {
     float *weights;
     char *dlogits;
     size_t tokens;
-    int n, k, groups, kept, lanes, score, renorm, vector;
+    int n, k, groups, kept, lanes, score, renorm, vector, vector_bias;
     int log_per;  // of a group's experts, -1 if they are no power of two
     float scale;
 };
@@ -199,8 +199,9 @@ __host__ __device__ inline int route_words(int span, int k, int groups) {
 enum { kAll, kEven, kUneven };
 
 template <class T, int Q, int GROUPS>
-__global__ __launch_bounds__(kThreads) void route_kernel(RouteArgs a) {
+__global__ __launch_bounds__(kThreads) void route_kernel(RouteArgs given) {
     extern __shared__ int lds[];
+    RouteArgs a = given;
     const int W = a.lanes, per_block = kThreads / W, t = threadIdx.x;
     const int lane = t & (W - 1), slot = t / W;
     const int e0 = lane * Q, span = W * Q;
@@ -210,6 +211,9 @@ __global__ __launch_bounds__(kThreads) void route_kernel(RouteArgs a) {
     const bool soft = a.score == TB_HIP_SCORE_SOFTMAX;
     for (size_t base = (size_t)blockIdx.x * per_block; base < a.tokens;
          base += (size_t)gridDim.x * per_block) {
+        // Conditions on these stay inside the loop, which seldom turns twice:
+        // kept over it they fill the scalar registers.
+        asm volatile("" : "+s"(a.n), "+s"(a.log_per), "+s"(a.groups));
         const size_t token = base + slot;
         const bool live = token < a.tokens && (!a.valid || a.valid[token]);
         const char *row = a.logits + token * a.stride;
@@ -232,11 +236,12 @@ __global__ __launch_bounds__(kThreads) void route_kernel(RouteArgs a) {
             inverse = 1.0f / lanes_sum(sum, W);
         }
         if (a.bias) {
+            float b[Q];
+            load_row<float, Q>(reinterpret_cast<const char *>(a.bias), e0, a.n, a.vector_bias, b);
 #pragma unroll
             for (int j = 0; j < Q; ++j) {
-                const float b = e0 + j < a.n ? a.bias[e0 + j] : 0.0f;
                 const float s = soft ? exp_of<true>(x[j] - top) * inverse : sigmoid_of<true>(x[j]);
-                key[j] = x[j] == -__builtin_inff() ? kGone : key_of(s + b);
+                key[j] = x[j] == -__builtin_inff() ? kGone : key_of(s + b[j]);
             }
         } else {
 #pragma unroll
@@ -454,8 +459,8 @@ __global__ __launch_bounds__(kThreads) void route_backward_kernel(RouteArgs a) {
 // in the segment.  Choices outside the experts count as expert n.  Up to
 // kSmallChoices one workgroup does all three.
 
-constexpr int kOrderWaves = 4, kSmallWaves = 16;
-constexpr int kBatch = 8;  // choices of a lane on their way at once
+constexpr int kOrderWaves = 4, kSmallWaves = 16, kSumThreads = 1024;
+constexpr int kBatch = 4;  // choices of a lane on their way at once
 constexpr size_t kSegment = 64 * kBatch, kMaxSegments = 4096, kSmallChoices = 8192;
 
 struct OrderArgs {
@@ -559,18 +564,18 @@ __global__ __launch_bounds__(kOrderWaves * 64) void order_count_kernel(OrderArgs
 }
 
 // One workgroup per expert: counts to exclusive running sums.
-__global__ __launch_bounds__(256) void order_sum_kernel(OrderArgs a) {
-    __shared__ int wave_total[4];
+__global__ __launch_bounds__(kSumThreads) void order_sum_kernel(OrderArgs a) {
+    __shared__ int wave_total[kSumThreads / 64];
     const int t = threadIdx.x, lane = t & 63;
     int *row = a.counts + (size_t)blockIdx.x * a.segments;
     int before = 0;
-    for (unsigned s0 = 0; s0 < a.segments; s0 += 256) {
+    for (unsigned s0 = 0; s0 < a.segments; s0 += kSumThreads) {
         const unsigned s = s0 + t;
         const int v = s < a.segments ? row[s] : 0, sum = running_sum(v);
         if (lane == 63) wave_total[t >> 6] = sum;
         __syncthreads();
         int below = 0, all = 0;
-        for (int w = 0; w < 4; ++w) {
+        for (int w = 0; w < kSumThreads / 64; ++w) {
             below += w < (t >> 6) ? wave_total[w] : 0;
             all += wave_total[w];
         }
@@ -669,8 +674,8 @@ unsigned grid_for(const RouteArgs &a) {
 }
 
 // Experts a lane.  Forward 16 above 16 experts, which halves what lanes do for
-// their token (163,840 tokens, us, 8 / 16 a lane: 4 of 64 20.5 / 15.6, 2 of 16
-// 6.8 / 7.0, 8 of 128 of 81,920 tokens 30.0 / 24.3); backward 8, which
+// their token (163,840 tokens, us, 8 / 16 a lane: 4 of 64 20.5 / 13.3, 2 of 16
+// 5.6 / 7.0, 8 of 128 of 81,920 tokens 30.0 / 22.5); backward 8, which
 // keeps more loads under way, as long as 64 lanes hold a token's.
 constexpr int kForwardEight = 16, kBackwardEight = 512;
 
@@ -755,6 +760,7 @@ extern "C" int tb_hip_route_device(const void *logits, size_t row_stride, const 
     (void)hipGetLastError();
     const bool eight = n_experts <= kForwardEight;
     a.vector = vector_rows(logits, row_stride, n_experts, eight ? 8 : 16);
+    a.vector_bias = vector_rows(bias, 0, n_experts, eight ? 8 : 16);
     with_type(dtype, [&](auto zero) {
         typedef decltype(zero) T;
         if (groups_kept == groups)
@@ -841,7 +847,7 @@ extern "C" int tb_hip_expert_order_device(const int *experts, const float *weigh
     }
     const unsigned blocks = (s.segments + kOrderWaves - 1) / kOrderWaves;
     order_count_kernel<<<blocks, kOrderWaves * 64, kOrderWaves * row, q>>>(a);
-    order_sum_kernel<<<n_experts + 1, 256, 0, q>>>(a);
+    order_sum_kernel<<<n_experts + 1, kSumThreads, 0, q>>>(a);
     order_place_kernel<<<blocks, kOrderWaves * 64, (1 + kOrderWaves) * row, q>>>(a);
     return hipGetLastError() == hipSuccess;
 }
