@@ -328,7 +328,6 @@ constexpr int kSlice = 2 * kPad, kSliceBytes = kSlice / 2;
 
 typedef const __attribute__((address_space(1))) void *GlobalPtr;
 typedef __attribute__((address_space(3))) void *LdsPtr;
-typedef __attribute__((address_space(3))) unsigned char *LdsBytes;
 
 __device__ __forceinline__ void load_to_lds(const void *from, void *to) {
     __builtin_amdgcn_global_load_lds((GlobalPtr)from, (LdsPtr)to, 16, 0, 0);
@@ -447,6 +446,7 @@ __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(ProductArgs a) {
     // Byte offset of each row's codes, by the loading wave, lane / 8 and load.
     __shared__ __attribute__((aligned(16))) unsigned row_code[kRows];
     __shared__ float scale_of_row[BM];
+    __shared__ __attribute__((aligned(16))) float bias_of[BN];
     __shared__ unsigned char real_row[BM];
 
     const int t = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t >> 6), lane = t & 63;
@@ -478,6 +478,7 @@ __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(ProductArgs a) {
     int row;
     if (t >= BM) {
         row = n0 + (t - BM) < a.n ? t - BM : (int)(a.n - 1 - n0);
+        bias_of[t - BM] = a.bias ? a.bias[w_first + n0 + row] : 0.0f;
     } else {
         const int in = t < height ? t : height - 1;
         row = a.rows ? a.rows[m0 + in] : in;
@@ -590,8 +591,7 @@ __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(ProductArgs a) {
     const size_t n1 = n0 + c;
     float bias[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-        bias[i] = a.bias && n1 + i < a.n ? a.bias[w_first + n1 + i] : 0.0f;
+    for (int i = 0; i < 8; ++i) bias[i] = bias_of[c + i];
 #pragma unroll
     for (int j0 = 0; j0 < MT; j0 += kPassTiles) {
         // The arrays in turn: a pass is read before the next but one is written.
