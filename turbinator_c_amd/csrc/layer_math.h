@@ -90,6 +90,17 @@ __device__ __forceinline__ float act_slope(float z) {
     return 1.0f;
 }
 
+// Sum over the wave's lanes up to this one: shifts within sixteen lanes, then
+// the last lane of the rows before.
+__device__ __forceinline__ int running_sum(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 15, 15, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 15, 15, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 15, 15, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 15, 15, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 10, 15, false);
+    return v + __builtin_amdgcn_update_dpp(0, v, 0x143, 12, 15, false);
+}
+
 // Calls f with the activation as a compile-time constant.
 template <int N>
 struct Int {

@@ -189,11 +189,7 @@ __device__ __forceinline__ bool find_rows(const ProductArgs &a, size_t tile, int
             hi = x < a.experts ? bound_of(a, x + 1) : a.m;
         }
         const unsigned tiles = hi > lo ? (unsigned)((hi - lo + height - 1) / height) : 0;
-        unsigned sum = tiles;
-        for (int off = 1; off < 64; off *= 2) {
-            const unsigned o = __shfl_up(sum, off);
-            if (lane >= off) sum += o;
-        }
+        const unsigned sum = (unsigned)running_sum((int)tiles);
         const unsigned long long reach = __ballot(tile < sum);
         if (reach) {
             const int at = __ffsll(reach) - 1;

@@ -124,18 +124,17 @@ __device__ __forceinline__ void load_row(const char *row, int e0, int n, int vec
 }
 
 // Whether all[i] is among the `kept` highest of all[count], ties to the lower
-// index.  Keys above kGone.
+// index.  Keys above kGone, and kGone behind the last up to a whole eight.
 __device__ __forceinline__ bool in_best(const int *all, int count, int i, int kept) {
     const int v = all[i];
     int before = 0;
-    for (int j0 = 0; j0 < count; j0 += 8) {
-        int other[8];  // read at once
+    for (int j0 = 0; j0 < count; j0 += 8)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) other[j] = j0 + j < count ? all[j0 + j] : kGone;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) before += other[j] > (j0 + j < i ? v - 1 : v);
-    }
+        for (int j = 0; j < 8; ++j) before += all[j0 + j] > (j0 + j < i ? v - 1 : v);
     return before < kept;
+}
+__device__ __forceinline__ void pad_standings(int *all, int count, int lane, int lanes) {
+    for (int i = count + lane; i < (count + 7) / 8 * 8; i += lanes) all[i] = kGone;
 }
 
 // The two best keys of a set.
@@ -155,36 +154,40 @@ __device__ __forceinline__ int standing(Two t, const float *bias) {
 }
 
 // The keys of the kept groups, groups of 2^log_per experts: the two best of
-// each in registers and between lanes, the standings through LDS.
-template <int Q>
+// each in registers and between lanes, the standings through LDS.  LOG is
+// log_per, Q's logarithm for groups of several lanes.
+template <int Q, int LOG>
 __device__ __forceinline__ void keep_groups(const RouteArgs &a, int e0, int lane, int *stands,
                                             int (&key)[Q]) {
+    constexpr int kStep = 1 << LOG;
     Two two[Q];
 #pragma unroll
     for (int j = 0; j < Q; ++j) two[j] = {key[j], kGone};
     // Leaders: the first of every group, or of the lane.
 #pragma unroll
-    for (int l = 0; (1 << l) < Q; ++l)
-        if (a.log_per > l) {
+    for (int l = 0; l < LOG; ++l)
 #pragma unroll
-            for (int j = 0; j < Q; j += 2 << l) two[j] = joined(two[j], two[j + (1 << l)]);
-        }
-    constexpr int kLogQ = Q == 8 ? 3 : 4;
-    const int share = a.log_per > kLogQ ? 1 << (a.log_per - kLogQ) : 1;  // lanes of a group
-    for (int off = 1; off < share; off *= 2)
-        two[0] = joined(two[0], Two{__shfl_xor(two[0].best, off), __shfl_xor(two[0].next, off)});
-    const int seg = a.log_per < kLogQ ? (1 << a.log_per) - 1 : Q - 1;
+        for (int j = 0; j < Q; j += 2 << l) two[j] = joined(two[j], two[j + (1 << l)]);
+    int share = 1;  // lanes of a group
+    if constexpr (kStep == Q) {
+        share = 1 << (a.log_per - LOG);
+        for (int off = 1; off < share; off *= 2)
+            two[0] =
+                joined(two[0], Two{__shfl_xor(two[0].best, off), __shfl_xor(two[0].next, off)});
+    }
 #pragma unroll
-    for (int j = 0; j < Q; ++j)
-        if ((j & seg) == 0 && e0 + j < a.n && (lane & (share - 1)) == 0)
+    for (int j = 0; j < Q; j += kStep)
+        if (e0 + j < a.n && (lane & (share - 1)) == 0)
             stands[(e0 + j) >> a.log_per] = standing(two[j], a.bias);
+    pad_standings(stands, a.groups, lane, a.lanes);
     wave_fence();
-    bool keep = false;
 #pragma unroll
-    for (int j = 0; j < Q; ++j) {
-        if ((j & seg) == 0)
-            keep = e0 + j < a.n && in_best(stands, a.groups, (e0 + j) >> a.log_per, a.kept);
-        if (!keep) key[j] = kGone;
+    for (int j = 0; j < Q; j += kStep) {
+        // Lanes past the last expert have no keys, and look at the first group.
+        const int g = e0 + j < a.n ? (e0 + j) >> a.log_per : 0;
+        const bool keep = in_best(stands, a.groups, g, a.kept);
+#pragma unroll
+        for (int i = j; i < j + kStep; ++i) key[i] = keep ? key[i] : kGone;
     }
 }
 
@@ -232,22 +235,35 @@ __global__ __launch_bounds__(kThreads) void route_kernel(RouteArgs given) {
             for (int j = 0; j < Q; ++j) top = fmaxf(top, x[j]);
             top = lanes_max(top, W);
 #pragma unroll
-            for (int j = 0; j < Q; ++j) sum += e0 + j < a.n ? exp_of<true>(x[j] - top) : 0.0f;
+            for (int j = 0; j < Q; ++j) sum += exp_of<true>(x[j] - top);  // -inf past the last
             inverse = 1.0f / lanes_sum(sum, W);
         }
         if (a.bias) {
             float b[Q];
             load_row<float, Q>(reinterpret_cast<const char *>(a.bias), e0, a.n, a.vector_bias, b);
+            if (soft) {
 #pragma unroll
-            for (int j = 0; j < Q; ++j) {
-                const float s = soft ? exp_of<true>(x[j] - top) * inverse : sigmoid_of<true>(x[j]);
-                key[j] = x[j] == -__builtin_inff() ? kGone : key_of(s + b[j]);
+                for (int j = 0; j < Q; ++j) b[j] += exp_of<true>(x[j] - top) * inverse;
+            } else {
+#pragma unroll
+                for (int j = 0; j < Q; ++j) b[j] += sigmoid_of<true>(x[j]);
             }
+#pragma unroll
+            for (int j = 0; j < Q; ++j)
+                key[j] = x[j] == -__builtin_inff() ? kGone : key_of(b[j]);
         } else {
 #pragma unroll
             for (int j = 0; j < Q; ++j) key[j] = key_of(x[j]);
         }
-        if constexpr (GROUPS == kEven) keep_groups<Q>(a, e0, lane, stands, key);
+        if constexpr (GROUPS == kEven) {
+            switch (a.log_per) {
+                case 0: keep_groups<Q, 0>(a, e0, lane, stands, key); break;
+                case 1: keep_groups<Q, 1>(a, e0, lane, stands, key); break;
+                case 2: keep_groups<Q, 2>(a, e0, lane, stands, key); break;
+                case 3: keep_groups<Q, 3>(a, e0, lane, stands, key); break;
+                default: keep_groups<Q, Q == 8 ? 3 : 4>(a, e0, lane, stands, key);
+            }
+        }
         if constexpr (GROUPS == kUneven) {
             const int per = a.n / a.groups;
 #pragma unroll
@@ -258,6 +274,7 @@ __global__ __launch_bounds__(kThreads) void route_kernel(RouteArgs given) {
                 for (int i = 0; i < per; ++i) two = joined(two, Two{keys[g * per + i], kGone});
                 stands[g] = standing(two, a.bias);
             }
+            pad_standings(stands, a.groups, lane, W);
             wave_fence();
             int g = e0 / per, left = per - (e0 - g * per);
             bool keep = g < a.groups && in_best(stands, a.groups, g, a.kept);
@@ -457,21 +474,22 @@ __global__ __launch_bounds__(kThreads) void route_backward_kernel(RouteArgs a) {
 // (2) for each expert the running sum over the segments, (3) the segments
 // again, each choice to its expert's start plus its running sum plus its rank
 // in the segment.  Choices outside the experts count as expert n.  Up to
-// kSmallChoices one workgroup does all three.
+// kSmallChoices one workgroup does all three (us, that / three launches, 64
+// experts: 640 choices 4.9 / 9.2, 4,000 7.9 / 9.8, 6,000 10.9 / 9.8).
 
 constexpr int kOrderWaves = 4, kSmallWaves = 16, kSumThreads = 1024;
 constexpr int kBatch = 4;  // choices of a lane on their way at once
-constexpr size_t kSegment = 64 * kBatch, kMaxSegments = 4096, kSmallChoices = 8192;
+constexpr size_t kSegment = 64 * kBatch, kMaxSegments = 4096, kSmallChoices = 5120;
 
 struct OrderArgs {
     const int *experts;
     const float *weights;
     int *offsets, *tokens, *positions;
     float *row_weights;
-    int *counts;  // [n + 1][segments], then their running sums
+    int *counts;  // [n + 1][padded], then their running sums
     int *totals;  // [n + 1]
     size_t choices, segment;
-    unsigned segments;
+    unsigned segments, padded;  // padded: to whole workgroups
     int n, k, bits;
 };
 
@@ -498,18 +516,30 @@ __device__ __forceinline__ void count_segment(const OrderArgs &a, size_t c0, siz
     }
 }
 
-// Writes a wave's segment; next[e] is the row of its next choice of expert e.
-__device__ __forceinline__ void place_segment(const OrderArgs &a, size_t c0, size_t c1,
-                                              int *next) {
-    const int lane = threadIdx.x & 63;
-    for (size_t cb = c0; cb < c1; cb += kSegment) {
-        int e[kBatch], row[kBatch];
+// A lane's choices of one turn, and their weights.
+struct Choices {
+    int e[kBatch];
+    float w[kBatch];
+    __device__ __forceinline__ void load(const OrderArgs &a, size_t cb, size_t c1) {
+        const int lane = threadIdx.x & 63;
         load_choices(a, cb, c1, e);
-        float w[kBatch];
         if (a.weights)
 #pragma unroll
             for (int j = 0; j < kBatch; ++j)
                 w[j] = cb + lane + 64 * j < c1 ? a.weights[cb + lane + 64 * j] : 0.0f;
+    }
+};
+
+// Writes a wave's segment; next[e] is the row of its next choice of expert e,
+// `now` holds the first choices.
+__device__ __forceinline__ void place_segment(const OrderArgs &a, size_t c0, size_t c1, int *next,
+                                              Choices now) {
+    const int lane = threadIdx.x & 63;
+    for (size_t cb = c0; cb < c1; cb += kSegment) {
+        int row[kBatch];
+        if (cb > c0) now.load(a, cb, c1);
+        const int(&e)[kBatch] = now.e;
+        const float(&w)[kBatch] = now.w;
 #pragma unroll
         for (int j = 0; j < kBatch; ++j) {
             const bool live = cb + lane + 64 * j < c1;
@@ -539,35 +569,34 @@ __device__ __forceinline__ void place_segment(const OrderArgs &a, size_t c0, siz
     }
 }
 
-// Sum over the lanes up to this one.
-__device__ __forceinline__ int running_sum(int v) {
-    const int lane = threadIdx.x & 63;
-    for (int off = 1; off < 64; off *= 2) {
-        const int o = __shfl_up(v, off);
-        if (lane >= off) v += o;
-    }
-    return v;
+// The counts of expert e in a workgroup's segments, those past the last too.
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+static_assert(kOrderWaves == 4);
+__device__ __forceinline__ i32x4 *counts_of(const OrderArgs &a, int e, unsigned block) {
+    return reinterpret_cast<i32x4 *>(a.counts + (size_t)e * a.padded) + block;
 }
 
 __global__ __launch_bounds__(kOrderWaves * 64) void order_count_kernel(OrderArgs a) {
     extern __shared__ int lds[];
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    int *count = lds + wave * (a.n + 1);
+    const int t = threadIdx.x, wave = t >> 6, lane = t & 63, columns = a.n + 1;
+    int *count = lds + wave * columns;
     const unsigned seg = blockIdx.x * kOrderWaves + wave;
-    if (seg >= a.segments) return;
-    for (int e = lane; e <= a.n; e += 64) count[e] = 0;
+    for (int e = lane; e < columns; e += 64) count[e] = 0;
     wave_fence();
     const size_t c0 = seg * a.segment;
-    count_segment(a, c0, c0 + a.segment < a.choices ? c0 + a.segment : a.choices, count);
-    wave_fence();
-    for (int e = lane; e <= a.n; e += 64) a.counts[(size_t)e * a.segments + seg] = count[e];
+    if (seg < a.segments)
+        count_segment(a, c0, c0 + a.segment < a.choices ? c0 + a.segment : a.choices, count);
+    __syncthreads();
+    for (int e = t; e < columns; e += kOrderWaves * 64)
+        *counts_of(a, e, blockIdx.x) = (i32x4){lds[e], lds[columns + e], lds[2 * columns + e],
+                                               lds[3 * columns + e]};
 }
 
 // One workgroup per expert: counts to exclusive running sums.
 __global__ __launch_bounds__(kSumThreads) void order_sum_kernel(OrderArgs a) {
     __shared__ int wave_total[kSumThreads / 64];
     const int t = threadIdx.x, lane = t & 63;
-    int *row = a.counts + (size_t)blockIdx.x * a.segments;
+    int *row = a.counts + (size_t)blockIdx.x * a.padded;
     int before = 0;
     for (unsigned s0 = 0; s0 < a.segments; s0 += kSumThreads) {
         const unsigned s = s0 + t;
@@ -590,9 +619,10 @@ __global__ __launch_bounds__(kSumThreads) void order_sum_kernel(OrderArgs a) {
 __device__ __forceinline__ void find_starts(const OrderArgs &a, const int *totals, int *start,
                                             bool write) {
     const int lane = threadIdx.x & 63;
-    int before = 0;
+    int before = 0, ahead = lane <= a.n ? totals[lane] : 0;
     for (int e0 = 0; e0 <= a.n; e0 += 64) {
-        const int e = e0 + lane, v = e <= a.n ? totals[e] : 0, sum = running_sum(v);
+        const int e = e0 + lane, v = ahead, sum = running_sum(v);
+        ahead = e + 64 <= a.n ? totals[e + 64] : 0;
         if (e <= a.n) {
             start[e] = before + sum - v;
             if (write) a.offsets[e] = before + sum - v;
@@ -604,16 +634,24 @@ __device__ __forceinline__ void find_starts(const OrderArgs &a, const int *total
 __global__ __launch_bounds__(kOrderWaves * 64) void order_place_kernel(OrderArgs a) {
     extern __shared__ int lds[];
     const int t = threadIdx.x, wave = t >> 6, lane = t & 63;
-    int *start = lds, *next = lds + (a.n + 1) * (1 + wave);
-    if (wave == 0) find_starts(a, a.totals, start, blockIdx.x == 0);
-    __syncthreads();
+    const int columns = a.n + 1;
+    int *start = lds, *next = lds + columns * (1 + wave);
     const unsigned seg = blockIdx.x * kOrderWaves + wave;
-    if (seg >= a.segments) return;
-    for (int e = lane; e <= a.n; e += 64)
-        next[e] = start[e] + a.counts[(size_t)e * a.segments + seg];
-    wave_fence();
     const size_t c0 = seg * a.segment;
-    place_segment(a, c0, c0 + a.segment < a.choices ? c0 + a.segment : a.choices, next);
+    const size_t c1 = c0 + a.segment < a.choices ? c0 + a.segment : a.choices;
+    Choices first;
+    first.load(a, c0, c1);  // on their way meanwhile
+    if (wave == 0) find_starts(a, a.totals, start, blockIdx.x == 0);
+    for (int e = t; e < columns; e += kOrderWaves * 64) {
+        const i32x4 before = *counts_of(a, e, blockIdx.x);
+#pragma unroll
+        for (int w = 0; w < kOrderWaves; ++w) lds[columns * (1 + w) + e] = before[w];
+    }
+    __syncthreads();
+    if (seg >= a.segments) return;
+    for (int e = lane; e < columns; e += 64) next[e] += start[e];
+    wave_fence();
+    place_segment(a, c0, c1, next, first);
 }
 
 // All of it in one workgroup: LDS holds the totals and each wave's counts.
@@ -625,6 +663,8 @@ __global__ __launch_bounds__(kSmallWaves * 64) void order_small_kernel(OrderArgs
     __syncthreads();
     const size_t c0 = wave * a.segment < a.choices ? wave * a.segment : a.choices;
     const size_t c1 = c0 + a.segment < a.choices ? c0 + a.segment : a.choices;
+    Choices first;
+    first.load(a, c0, c1);
     count_segment(a, c0, c1, next);
     __syncthreads();
     // Counts to running sums over the waves; the totals behind.
@@ -645,7 +685,7 @@ __global__ __launch_bounds__(kSmallWaves * 64) void order_small_kernel(OrderArgs
         lds[columns + i] += start[e];
     }
     __syncthreads();
-    place_segment(a, c0, c1, next);
+    place_segment(a, c0, c1, next, first);
 }
 
 // --------------------------------------------------------------------------
@@ -711,7 +751,7 @@ void with_type(int dtype, F f) {
 
 struct OrderShape {
     size_t segment;
-    unsigned segments;
+    unsigned segments, blocks;
 };
 
 OrderShape order_shape(size_t choices) {
@@ -720,6 +760,7 @@ OrderShape order_shape(size_t choices) {
     const size_t least = (choices + kMaxSegments - 1) / kMaxSegments;
     if (least > s.segment) s.segment = (least + 63) / 64 * 64;
     s.segments = (unsigned)((choices + s.segment - 1) / s.segment);
+    s.blocks = (s.segments + kOrderWaves - 1) / kOrderWaves;
     return s;
 }
 
@@ -810,7 +851,7 @@ extern "C" int tb_hip_route_backward_device(const void *logits, size_t row_strid
 extern "C" size_t tb_hip_expert_order_workspace_bytes(size_t tokens, int n_experts, int k) {
     if (!order_ok(tokens, n_experts, k)) return 0;
     const OrderShape s = order_shape(tokens * k);
-    const size_t ints = (size_t)(n_experts + 1) * (s.segments + 1);
+    const size_t ints = (size_t)(n_experts + 1) * (s.blocks * kOrderWaves + 1);
     return (ints * sizeof(int) + 15) & ~size_t(15);
 }
 
@@ -830,7 +871,8 @@ extern "C" int tb_hip_expert_order_device(const int *experts, const float *weigh
     a.positions = positions;
     a.row_weights = row_weights;
     a.counts = static_cast<int *>(workspace);
-    a.totals = a.counts + (size_t)(n_experts + 1) * s.segments;
+    a.padded = s.blocks * kOrderWaves;
+    a.totals = a.counts + (size_t)(n_experts + 1) * a.padded;
     a.choices = tokens * k;
     a.segment = s.segment;
     a.segments = s.segments;
@@ -845,9 +887,8 @@ extern "C" int tb_hip_expert_order_device(const int *experts, const float *weigh
         order_small_kernel<<<1, kSmallWaves * 64, row * (1 + kSmallWaves), q>>>(a);
         return hipGetLastError() == hipSuccess;
     }
-    const unsigned blocks = (s.segments + kOrderWaves - 1) / kOrderWaves;
-    order_count_kernel<<<blocks, kOrderWaves * 64, kOrderWaves * row, q>>>(a);
+    order_count_kernel<<<s.blocks, kOrderWaves * 64, kOrderWaves * row, q>>>(a);
     order_sum_kernel<<<n_experts + 1, kSumThreads, 0, q>>>(a);
-    order_place_kernel<<<blocks, kOrderWaves * 64, (1 + kOrderWaves) * row, q>>>(a);
+    order_place_kernel<<<s.blocks, kOrderWaves * 64, (1 + kOrderWaves) * row, q>>>(a);
     return hipGetLastError() == hipSuccess;
 }
