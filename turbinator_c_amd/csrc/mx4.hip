@@ -406,24 +406,20 @@ __device__ __forceinline__ void multiply(const Operands<MT, NT> &o, f32x4 (&acc)
                                 acc[i][j]);
 }
 
-// Eight consecutive columns n0 .. of row r.
+// 16 bytes of columns from n0 on of row r.  Nothing here reads them again:
+// stores past the caches (8,192 x 2,048 results, k 1,024: 20.7 us, else 22.4).
 template <class T>
-__device__ __forceinline__ void store8(const ProductArgs &a, size_t r, size_t n0,
-                                       const float (&v)[8]) {
+__device__ __forceinline__ void store_run(const ProductArgs &a, size_t r, size_t n0, u32x4 run) {
+    constexpr int kRun = 16 / sizeof(T);
     T *out = reinterpret_cast<T *>(a.out) + r * a.n + n0;
-    if (a.vector && n0 + 8 <= a.n) {
-        typedef Vec<T, 16> X;
-#pragma unroll
-        for (int p = 0; p < 8 / X::n; ++p) {
-            float part[X::n];
-#pragma unroll
-            for (int i = 0; i < X::n; ++i) part[i] = v[p * X::n + i];
-            *reinterpret_cast<typename X::raw *>(out + p * X::n) = X::pack(part);
-        }
+    if (a.vector) {  // rows hold whole runs
+        __builtin_nontemporal_store(run, reinterpret_cast<u32x4 *>(out));
     } else {
+        typedef T elems __attribute__((ext_vector_type(kRun)));
+        const elems v = __builtin_bit_cast(elems, run);
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (n0 + i < a.n) out[i] = (T)v[i];
+        for (int i = 0; i < kRun; ++i)
+            if (n0 + i < a.n) out[i] = v[i];
     }
 }
 
@@ -461,10 +457,10 @@ __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(ProductArgs a) {
     const size_t w_first = none ? 0 : (size_t)rt.expert * a.n;
 
     if (none) {
-        const float zeros[8] = {};
-        const size_t c = n0 + t % (BN / 8) * 8;
-        for (int r = t / (BN / 8); r < height; r += kThreads * 8 / BN)
-            if (c < a.n) store8<T>(a, m0 + r, c, zeros);
+        constexpr int kRun = 16 / sizeof(T), kAcross = BN / kRun;
+        const size_t c = n0 + t % kAcross * kRun;
+        for (int r = t / kAcross; r < height; r += kThreads / kAcross)
+            if (c < a.n) store_run<T>(a, m0 + r, c, (u32x4){0, 0, 0, 0});
         return;
     }
     // The matrix row behind each row of the tile, the output's rows first,
@@ -578,42 +574,50 @@ __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(ProductArgs a) {
     }
     arrive();
 
-    // Sums through LDS, so that a thread finishes eight columns of its own,
-    // the same for all its rows: kPass rows of the tile at a time.
-    constexpr int kPitch = BN + 4;
-    constexpr int kPassTiles = pass_tiles(MT, WM * 16 * kPitch * 4, sizeof(codes0));
-    constexpr int kPass = kPassTiles * WM * 16, kSweep = kThreads * 8 / BN;
-    const int c = t % (BN / 8) * 8;
+    // Results through LDS, whose rows leave in runs: kPass rows of the tile at a
+    // time, the arrays in turn, so that a pass is read before the next but one
+    // is written.  A lane's four columns are one piece; piece c of a wave's row
+    // r lies at c ^ 4 r, so that the rows of a write fall on different banks.
+    typedef Vec<T, 4 * sizeof(T)> Four;
+    constexpr int kPassTiles = pass_tiles(MT, WM * 16 * BN * sizeof(T), sizeof(codes0));
+    constexpr int kPass = kPassTiles * WM * 16, kPieces = BN / 4;
+    constexpr int kRun = 16 / sizeof(T), kAcross = BN / kRun, kSweep = kThreads / kAcross;
+    const int c = t % kAcross * kRun;
     const size_t n1 = n0 + c;
-    float bias[8];
+    f32x4 bias[NT];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) bias[i] = bias_of[c + i];
+    for (int i = 0; i < NT; ++i)
+        bias[i] = *reinterpret_cast<const f32x4 *>(bias_of + (wn * NT + i) * 16 + part * 4);
 #pragma unroll
     for (int j0 = 0; j0 < MT; j0 += kPassTiles) {
-        // The arrays in turn: a pass is read before the next but one is written.
-        float *sums = reinterpret_cast<float *>(j0 / kPassTiles % 2 ? codes1 : codes0);
+        unsigned char *results = j0 / kPassTiles % 2 ? codes1 : codes0;
 #pragma unroll
-        for (int j = 0; j < kPassTiles; ++j)
+        for (int j = 0; j < kPassTiles; ++j) {
+            const int in = (wm * MT + j0 + j) * 16 + low, at = (wm * kPassTiles + j) * 16 + low;
+            const float scale = scale_of_row[in];
+            const bool real = real_row[in];
 #pragma unroll
-            for (int i = 0; i < NT; ++i)
-                *reinterpret_cast<f32x4 *>(sums + ((wm * kPassTiles + j) * 16 + low) * kPitch +
-                                           (wn * NT + i) * 16 + part * 4) = acc[i][j0 + j];
+            for (int i = 0; i < NT; ++i) {
+                float v[4];
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    v[q] = act_of<kFine<T>, ACT>(acc[i][j0 + j][q] + bias[i][q]) * scale;
+                    v[q] = real ? v[q] : 0.0f;
+                }
+                const int piece = ((wn * NT + i) * 4 + part) ^ (low * 4 & (kPieces - 1));
+                reinterpret_cast<typename Four::raw *>(results)[at * kPieces + piece] =
+                    Four::pack(v);
+            }
+        }
         __syncthreads();
         if (n1 >= a.n) continue;
 #pragma unroll 4
-        for (int row = t / (BN / 8); row < kPass; row += kSweep) {
+        for (int row = t / kAcross; row < kPass; row += kSweep) {
             const int in = row / (kPassTiles * 16) * (MT * 16) + j0 * 16 + row % (kPassTiles * 16);
-            const f32x4 lo = *reinterpret_cast<const f32x4 *>(sums + row * kPitch + c);
-            const f32x4 hi = *reinterpret_cast<const f32x4 *>(sums + row * kPitch + c + 4);
-            const float scale = scale_of_row[in];
-            const bool real = real_row[in];
-            float v[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float z = (i < 4 ? lo[i & 3] : hi[i & 3]) + bias[i];
-                v[i] = real ? act_of<kFine<T>, ACT>(z) * scale : 0.0f;
-            }
-            if (in < height) store8<T>(a, m0 + in, n1, v);
+            const int piece = c / 4 ^ (row % 16 * 4 & (kPieces - 1));
+            const u32x4 run = *reinterpret_cast<const u32x4 *>(
+                results + (row * kPieces + piece) * sizeof(typename Four::raw));
+            if (in < height) store_run<T>(a, m0 + in, n1, run);
         }
     }
 }
@@ -633,19 +637,19 @@ size_t tiles_of(const ProductArgs &a, int shape) {
 }
 
 // Measured (us; large / middle / few rows with 4, 2 and 1 row tiles; bf16 out):
-//   m 16,384 n 4,096 k 4,096: 188 / 270 / 2,230 / 2,675 / -
-//   m  8,192 n 2,048 k 1,024: 20.3 / 25.8 / 197 / 209 / 260     (256 large tiles)
-//   m 16,384 n   512 k   512: 15.1 / 12.0 / 55 / 63 / 92        (128 large tiles)
-//   m    320 n 2,048 k 2,048: 19.3 / 12.0 / 18.6 / 17.3 / 23.0
-//   m    128 n 4,096 k 4,096: 28.3 / 18.7 / 21.7 / 25.1 / 32.1
-//   m     64 n 4,096 k 4,096: 26.9 / 17.3 / 12.7 / 14.4 / 17.8
-//   m     64 n 1,024 k 1,024: 12.0 / 7.9 / 6.1 / 5.0 / 4.3
-//   m     10 n 2,048 k 2,048: 16.3 / 10.1 / 5.7 / 5.2 / 4.9
+//   m 16,384 n 4,096 k 4,096: 189 / 254 / 2,230 / 2,677 / -
+//   m  8,192 n 2,048 k 1,024: 18.3 / 21.8 / 191 / 199 / 238     (256 large tiles)
+//   m 16,384 n   512 k   512: 12.6 / 10.1 / 56 / 56 / 71        (128 large tiles)
+//   m    320 n 2,048 k 2,048: 18.1 / 10.7 / 18.0 / 17.0 / 21.4
+//   m    128 n 4,096 k 4,096: 27.9 / 17.1 / 21.3 / 24.6 / 31.7
+//   m     64 n 4,096 k 4,096: 27.4 / 16.3 / 12.4 / 13.8 / 17.5
+//   m     64 n 1,024 k 1,024: 12.1 / 7.3 / 5.6 / 4.5 / 3.9
+//   m     10 n 2,048 k 2,048: 16.8 / 9.8 / 5.3 / 4.8 / 4.4
 // So: staged tiles where the output has more than 2^18 values (a lone staged
 // tile takes about 0.7 us for 256 values of k, the few-row kernel about 3 ns
 // for a thousand outputs) and experts fill more than a quarter of a middle
 // tile; large ones, one to a CU, or middle ones, two to a CU, by what a round
-// of them takes, 8.2 + 2.4 and 4.3 + 1.8 us for each slice of k (from the
+// of them takes, 8.2 + 2.4 and 3.9 + 1.8 us for each slice of k (from the
 // lines above).  Else as many row tiles as leave a workgroup to every CU.
 int shape_for(const ProductArgs &a) {
     // The staged kernels address a matrix with 32 bits from a tile's first row
@@ -658,7 +662,7 @@ int shape_for(const ProductArgs &a) {
         const size_t slices = (a.kp + kSlice - 1) / kSlice, ends = a.experts / 2;
         const size_t large = ((a.m + 255) / 256 + ends) * ((a.n + 255) / 256);
         const size_t middle = ((a.m + 127) / 128 + ends) * ((a.n + 127) / 128);
-        return (large + 255) / 256 * (82 + 24 * slices) <= (middle + 511) / 512 * (43 + 18 * slices)
+        return (large + 255) / 256 * (82 + 24 * slices) <= (middle + 511) / 512 * (39 + 18 * slices)
                    ? kLarge
                    : kMiddle;
     }
