@@ -34,6 +34,7 @@ constexpr size_t kMaxCount = 0x7fffffffu;
 constexpr int kThreads = 512;      // of a workgroup; kMaxThreads where a pixel has more lanes
 constexpr int kMaxThreads = 1024;
 constexpr int kVectors = 8;        // a chunk holds this many vectors a thread
+constexpr int kAhead = 4;          // of them a thread loads before it uses the first
 constexpr size_t kMaxGrid = 1 << 20;
 
 // How a launch divides the planes.
@@ -160,7 +161,10 @@ __device__ __forceinline__ Place place_of(const NormArgs &a, size_t item) {
 
 // Mean and sum of squared deviations of each group over one chunk.  A sweep
 // of kVectors vectors a thread stays in registers for both; sweeps of a longer
-// chunk are joined with Chan's formula.
+// chunk are joined with Chan's formula.  Bound by memory, which the second
+// launch reads again, from the last cache where the planes fit it: both take
+// 77 us for 16 x 65,536 x 64 bf16 (3.5 TB/s of x and y), 334 us for 128 x
+// 16,384 x 128 (3.2).
 template <class T, int B>
 __global__ __launch_bounds__(kMaxThreads) void norm_parts_kernel(NormArgs a) {
     typedef Vec<T, B> X;
@@ -297,14 +301,26 @@ __global__ __launch_bounds__(kMaxThreads) void norm_apply_kernel(NormArgs a) {
             }
             const char *x = a.x + w.image * a.x_image + (size_t)c0 * sizeof(T);
             char *y = a.out + (w.image * a.pixels * a.channels + c0) * sizeof(T);
-            for (unsigned p = w.p0 + row; p < w.p1; p += s.rows) {
-                float v[V];
-                X::unpack(*reinterpret_cast<const typename X::raw *>(x + p * a.x_pixel), v);
+            for (unsigned p0 = w.p0 + row; p0 < w.p1; p0 += s.rows * kAhead) {
+                typename X::raw raw[kAhead];
 #pragma unroll
-                for (int i = 0; i < V; ++i)
-                    v[i] = act_of<kFine<T>, ACT>(fmaf(v[i] - mean[i], scale[i], shift[i]));
-                *reinterpret_cast<typename X::raw *>(y + (size_t)p * a.channels * sizeof(T)) =
-                    X::pack(v);
+                for (int j = 0; j < kAhead; ++j) {
+                    const unsigned p = p0 + j * s.rows;
+                    if (p < w.p1)
+                        raw[j] = *reinterpret_cast<const typename X::raw *>(x + p * a.x_pixel);
+                }
+#pragma unroll
+                for (int j = 0; j < kAhead; ++j) {
+                    const unsigned p = p0 + j * s.rows;
+                    if (p >= w.p1) break;
+                    float v[V];
+                    X::unpack(raw[j], v);
+#pragma unroll
+                    for (int i = 0; i < V; ++i)
+                        v[i] = act_of<kFine<T>, ACT>(fmaf(v[i] - mean[i], scale[i], shift[i]));
+                    *reinterpret_cast<typename X::raw *>(y + (size_t)p * a.channels * sizeof(T)) =
+                        X::pack(v);
+                }
             }
         }
         __syncthreads();
@@ -345,8 +361,38 @@ struct Channels {
     }
 };
 
+// f(pixel, u, d) of a thread's vectors of a chunk, kAhead of them loaded at once.
+template <class T, int B, int ACT, class F>
+__device__ __forceinline__ void grad_sweep(const NormArgs &a, const Place &w, int row,
+                                           const char *x, const char *dy,
+                                           const Channels<Vec<T, B>::n> &ch, F f) {
+    typedef Vec<T, B> X;
+    const int rows = a.s.rows;
+    for (unsigned p0 = w.p0 + row; p0 < w.p1; p0 += rows * kAhead) {
+        typename X::raw xr[kAhead], gr[kAhead];
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) {
+            const unsigned p = p0 + j * rows;
+            if (p < w.p1) {
+                xr[j] = *reinterpret_cast<const typename X::raw *>(x + p * a.x_pixel);
+                gr[j] = *reinterpret_cast<const typename X::raw *>(dy + p * a.dy_pixel);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) {
+            const unsigned p = p0 + j * rows;
+            if (p >= w.p1) break;
+            float u[X::n], d[X::n];
+            grad_terms<T, B, ACT>(xr[j], gr[j], ch.mean, ch.scale, ch.beta, u, d);
+            f(p, u, d);
+        }
+    }
+}
+
 // The sums of u and u h of every channel over one chunk:
-// parts[(image, chunk)][channel][2].
+// parts[(image, chunk)][channel][2].  With grad_apply_kernel 176 us for 16 x
+// 65,536 x 64 bf16 (2.3 TB/s of x, dy and dx, five passes for three), 550 us
+// for 128 x 16,384 x 128 (2.9).
 template <class T, int B, int ACT>
 __global__ __launch_bounds__(kMaxThreads) void grad_parts_kernel(NormArgs a) {
     typedef Vec<T, B> X;
@@ -368,18 +414,14 @@ __global__ __launch_bounds__(kMaxThreads) void grad_parts_kernel(NormArgs a) {
             ch.load(a, w.image, c0);
             const char *x = a.x + w.image * a.x_image + (size_t)c0 * sizeof(T);
             const char *dy = a.dy + w.image * a.dy_image + (size_t)c0 * sizeof(T);
-            for (unsigned p = w.p0 + row; p < w.p1; p += s.rows) {
-                float u[V], d[V];
-                grad_terms<T, B, ACT>(
-                    *reinterpret_cast<const typename X::raw *>(x + p * a.x_pixel),
-                    *reinterpret_cast<const typename X::raw *>(dy + p * a.dy_pixel), ch.mean,
-                    ch.scale, ch.beta, u, d);
+            grad_sweep<T, B, ACT>(a, w, row, x, dy, ch,
+                                  [&](unsigned, const float(&u)[V], const float(&d)[V]) {
 #pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    su[i] += u[i];
-                    sh[i] = fmaf(u[i], d[i], sh[i]);
-                }
-            }
+                                      for (int i = 0; i < V; ++i) {
+                                          su[i] += u[i];
+                                          sh[i] = fmaf(u[i], d[i], sh[i]);
+                                      }
+                                  });
 #pragma unroll
             for (int i = 0; i < V; ++i) sh[i] *= ch.rstd[i];
         }
@@ -400,6 +442,11 @@ __global__ __launch_bounds__(kMaxThreads) void grad_parts_kernel(NormArgs a) {
     }
 }
 
+typedef float Pair __attribute__((ext_vector_type(2)));
+__host__ __device__ __forceinline__ int shares_of(const Shape &s) {
+    return s.threads > s.slab ? s.threads / s.slab : 1;
+}
+
 template <class T, int B, int ACT>
 __global__ __launch_bounds__(kMaxThreads) void grad_apply_kernel(NormArgs a) {
     typedef Vec<T, B> X;
@@ -407,18 +454,34 @@ __global__ __launch_bounds__(kMaxThreads) void grad_apply_kernel(NormArgs a) {
     extern __shared__ float lds[];
     const Shape s = a.s;
     const int t = threadIdx.x, wave = t >> 6, waves = blockDim.x >> 6;
-    float *m1 = lds, *m2 = lds + s.slab;
+    const int shares = shares_of(s);
+    float *m1 = lds, *m2 = m1 + s.slab, *sum1 = m2 + s.slab, *sum2 = sum1 + s.slab * shares;
     const int lane = t % s.lanes, row = t / s.lanes;
     const size_t items = a.images * s.slabs * s.chunks;
     const float inverse = 1.0f / ((float)a.pixels * a.per);
     for (size_t item = blockIdx.x; item < items; item += gridDim.x) {
         const Place w = place_of(a, xcd_contiguous(item, items));
-        for (int c = t; c < s.slab; c += blockDim.x) {
-            const float *at = a.parts + (w.image * s.chunks * a.channels + w.c0 + c) * 2;
+        // A channel's chunks are summed by `shares` threads, then those sums.
+        for (int i = t; i < s.slab * shares; i += blockDim.x) {
+            const int share = i / s.slab, c = i - share * s.slab;
+            const Pair *at = reinterpret_cast<const Pair *>(a.parts) +
+                             w.image * s.chunks * a.channels + w.c0 + c;
             float one = 0.0f, two = 0.0f;
-            for (unsigned i = 0; i < s.chunks; ++i) {
-                one += at[(size_t)i * a.channels * 2];
-                two += at[(size_t)i * a.channels * 2 + 1];
+#pragma unroll 4
+            for (unsigned j = share; j < s.chunks; j += shares) {
+                const Pair v = at[(size_t)j * a.channels];
+                one += v[0];
+                two += v[1];
+            }
+            sum1[i] = one;
+            sum2[i] = two;
+        }
+        __syncthreads();
+        for (int c = t; c < s.slab; c += blockDim.x) {
+            float one = 0.0f, two = 0.0f;
+            for (int i = 0; i < shares; ++i) {
+                one += sum1[i * s.slab + c];
+                two += sum2[i * s.slab + c];
             }
             const float gamma = a.gamma ? a.gamma[w.c0 + c] : 1.0f;
             m1[c] = one * gamma;
@@ -448,18 +511,15 @@ __global__ __launch_bounds__(kMaxThreads) void grad_apply_kernel(NormArgs a) {
                 less[i] = ch.rstd[i] * m1[lane * V + i];
                 slope[i] = ch.rstd[i] * ch.rstd[i] * m2[lane * V + i];
             }
-            for (unsigned p = w.p0 + row; p < w.p1; p += s.rows) {
-                float u[V], d[V];
-                grad_terms<T, B, ACT>(
-                    *reinterpret_cast<const typename X::raw *>(x + p * a.x_pixel),
-                    *reinterpret_cast<const typename X::raw *>(dy + p * a.dy_pixel), ch.mean,
-                    ch.scale, ch.beta, u, d);
+            grad_sweep<T, B, ACT>(
+                a, w, row, x, dy, ch, [&](unsigned p, const float(&u)[V], const float(&d)[V]) {
+                    float v[V];
 #pragma unroll
-                for (int i = 0; i < V; ++i)
-                    u[i] = fmaf(-d[i], slope[i], fmaf(u[i], ch.scale[i], -less[i]));
-                *reinterpret_cast<typename X::raw *>(dx + (size_t)p * a.channels * sizeof(T)) =
-                    X::pack(u);
-            }
+                    for (int i = 0; i < V; ++i)
+                        v[i] = fmaf(-d[i], slope[i], fmaf(u[i], ch.scale[i], -less[i]));
+                    *reinterpret_cast<typename X::raw *>(
+                        dx + (size_t)p * a.channels * sizeof(T)) = X::pack(v);
+                });
         }
         __syncthreads();
     }
@@ -467,7 +527,9 @@ __global__ __launch_bounds__(kMaxThreads) void grad_apply_kernel(NormArgs a) {
 
 // Planes whose slab fits the registers of one workgroup: one pass over memory.
 // Every thread holds NV vectors; the means, then the squared deviations, then
-// the elements come from them.
+// the elements come from them.  4,096 x 1,024 x 64 bf16 with SiLU: 250 us, 4.3
+// TB/s of x and y, where a copy of 4 GiB moves 4.8; 257 x 1,023 x 48 fp32 with
+// GELU: 32 us, 3.2 TB/s, 771 workgroups on 256 CUs.
 template <class T, int B, int NV, int ACT>
 __global__ __launch_bounds__(kMaxThreads) void norm_whole_kernel(NormArgs a) {
     typedef Vec<T, B> X;
@@ -565,6 +627,10 @@ __global__ __launch_bounds__(kMaxThreads) void norm_whole_kernel(NormArgs a) {
 // sums and the elements.  A workgroup takes every so manieth image of its slab
 // and keeps its channels' sums: parts[workgroup of the slab][channel][2].
 // What belongs to a channel is formed by one thread and read from LDS.
+// 1,024 x 2,048 x 64 bf16 with SiLU: 244 us, 3.3 TB/s of x, dy and dx.  A
+// plane's x and dy take half of a CU's registers, so one workgroup has the CU
+// and its loads, sums and stores take turns; reading both twice, with two to
+// four workgroups to a CU, took 240 to 298 us.
 template <class T, int B, int NV, int ACT>
 __global__ __launch_bounds__(kMaxThreads) void grad_whole_kernel(NormArgs a) {
     typedef Vec<T, B> X;
@@ -680,7 +746,8 @@ __global__ __launch_bounds__(kMaxThreads) void grad_whole_kernel(NormArgs a) {
 
 // parts[rows][channels][2] summed over the rows of each of gridDim.y spans:
 // to `parts` of the next level, or to dbeta and dgamma.  32 channels and 32
-// rows at a time a workgroup.
+// rows at a time a workgroup: 4.6 us for 128 rows of 64 channels, a launch's
+// time.
 constexpr int kSumChannels = 32, kSumRows = 32;
 
 __global__ __launch_bounds__(kSumChannels *kSumRows) void grad_sum_kernel(
@@ -870,7 +937,8 @@ void launch_backward(const NormArgs &a, hipStream_t q) {
     if constexpr (B != 8) {
         const unsigned grid = (unsigned)grid_of(a);
         grad_parts_kernel<T, B, ACT><<<grid, s.threads, 2 * part, q>>>(a);
-        grad_apply_kernel<T, B, ACT><<<grid, s.threads, 2 * slab, q>>>(a);
+        grad_apply_kernel<T, B, ACT>
+            <<<grid, s.threads, 2 * slab * (1 + shares_of(s)), q>>>(a);
     }
 }
 
