@@ -1,9 +1,6 @@
 // Group norm with an activation over channels-last planes, forward and
-// backward (hip_layers.h).  The reference's stems normalise its planes with
-// kernels of their own (groupnorm_stats, _apply and _backward of
-// src/network/network_gpu.cu, channels first); here the activation is in the
-// same pass and the planes are channels last, as a matrix-core convolution
-// leaves them.
+// backward (hip_layers.h).  The activation is in the same pass, and the planes
+// are channels last, as a matrix-core convolution leaves them.
 //
 //   h = (x - mean) rstd,  z = h gamma + beta,  y = act(z)
 //   u = dy act'(z):  dbeta = sum u,  dgamma = sum u h  (images, pixels)

@@ -1,7 +1,7 @@
 // Microscaled 4-bit floating point (hip_layers.h): quantisation, the values it
-// stands for, and products on the scaled matrix instructions.  The reference's
-// actor multiplies in fp32 through a library; acting reads far more weights
-// than it multiplies, so a quarter of bf16's bytes is what this form is for.
+// stands for, and products on the scaled matrix instructions.  Acting on a few
+// tokens reads far more weights than it multiplies: a quarter of bf16's bytes
+// is what this form is for.
 //
 //   scale  2^(s - 127), s = max(exponent bits of the largest magnitude - 2, 0)
 //   code   value / scale (exact: a power of two) rounded to 0, 0.5, 1, 1.5, 2,
@@ -327,7 +327,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_kernel(ProductArgs a) {
 //
 // m 16,384, n 4,096, k 4,096: 178 to 189 us, 2.9 to 3.1 PFLOP/s, half of what
 // the instruction does from registers on such values (6.4): the waves of a CU
-// meet at a barrier every 128 instructions.  At short k the ends count: k
+// meet at a barrier every 64 matrix instructions.  At short k the ends count: k
 // 1,024 takes 18.3 us for 8,192 x 2,048, of which 8 are starting and storing.
 constexpr int kSlice = 2 * kPad, kSliceBytes = kSlice / 2;
 

@@ -1,8 +1,6 @@
 // Routing of tokens to experts, its gradient, and the order of the choices by
-// expert (hip_layers.h).  The reference's actor mixes the two best experts of
-// every token densely (moe_mix, src/network/network_gpu.cu:373-390); here the
-// choice leaves as indices and weights, so each expert's product runs on its
-// own tokens only.
+// expert (hip_layers.h).  The choice leaves as indices and weights, so each
+// expert's product runs on its own tokens only.
 //
 //   s = softmax(l) or sigmoid(l);  key = l, or s + b with a bias
 //   w_i = scale s_i, renormalised scale s_i / S, S the sum over the chosen
