@@ -51,8 +51,9 @@ enum {
  * Returns 0 for NULL x or y, a workspace that is NULL or misaligned,
  * images, pixels, channels or groups 0 or images or pixels above 0x7fffffff,
  * channels above TB_HIP_NORM_MAX_CHANNELS or not a multiple of groups, a group
- * above TB_HIP_NORM_MAX_GROUP channels, x, y or strides that are not multiples of the element's size, an
- * unknown act or dtype, or an eps that is not positive and finite. */
+ * above TB_HIP_NORM_MAX_GROUP channels, x, y or strides that are not multiples
+ * of the element's size, an unknown act or dtype, or an eps that is not
+ * positive and finite. */
 int tb_hip_group_norm_device(const void *x, size_t image_stride, size_t pixel_stride,
                              const float *gamma, const float *beta, void *y, float *mean,
                              float *rstd, void *workspace, size_t images, size_t pixels,

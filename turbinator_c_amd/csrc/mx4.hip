@@ -443,7 +443,8 @@ __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(ProductArgs a) {
     // of one need not wait for the loads into the other.
     __shared__ __attribute__((aligned(1024))) unsigned char codes0[kRows * kSliceBytes];
     __shared__ __attribute__((aligned(1024))) unsigned char codes1[kRows * kSliceBytes];
-    __shared__ __attribute__((aligned(4096))) int scales0[kRows * 2], scales1[kRows * 2];  // [group of 64 rows][step][lane]
+    // [group of 64 rows][step][lane]
+    __shared__ __attribute__((aligned(4096))) int scales0[kRows * 2], scales1[kRows * 2];
     // Byte offset of each row's codes, by the loading wave, lane / 8 and load.
     __shared__ __attribute__((aligned(16))) unsigned row_code[kRows];
     __shared__ float scale_of_row[BM];
