@@ -69,11 +69,40 @@ __device__ __forceinline__ float sigmoid_of(float z) {
     return __builtin_amdgcn_rcpf(1.0f + exp_of<FINE>(-z));
 }
 
+// The normal distribution below z, and e^(-z^2/2) on the way.  Below 0 it is
+// erfc(|z| / sqrt 2) / 2 in the form e^(-z^2/2) t P(t), t = 1 / (1 + 0.21 |z|)
+// (Abramowitz and Stegun 7.1.26's, with a longer P): relative digits stay as
+// far as the result is a normal number, where 1 + erf(z / sqrt 2) cancels (4%
+// of GELU off at -5, all of it from -6 on).  P is the polynomial of degree 8
+// with the least relative error, 0.2 units of 2^-24, for |z| up to 13.3, from
+// where on the exponential is 0 or subnormal; with it the result is within 12
+// units for z above -3 and z^2 (16-bit results: 2 z^2) further out.
+// 4,096 x 1,024 x 64 bf16 through GELU in group norm, forward: 292 us, and 451
+// with erfcf; gradient of 1,024 x 2,048 x 64: 318 and 505.
+struct Normal {
+    float below, bell;
+};
+template <bool FINE>
+__device__ __forceinline__ Normal normal_of(float z) {
+    const float bell = exp_of<FINE>(-0.5f * z * z);
+    const float t = __builtin_amdgcn_rcpf(fmaf(0.21f, __builtin_fabsf(z), 1.0f));
+    float p = -0.072194494f;
+    p = fmaf(p, t, 0.2862464f);
+    p = fmaf(p, t, -0.3358655f);
+    p = fmaf(p, t, 0.35600975f);
+    p = fmaf(p, t, -0.09866595f);
+    p = fmaf(p, t, 0.12699148f);
+    p = fmaf(p, t, 0.068616636f);
+    p = fmaf(p, t, 0.085155666f);
+    p = fmaf(p, t, 0.083706014f);
+    const float tail = p * t * bell;
+    return {z < 0.0f ? tail : 1.0f - tail, bell};
+}
+
 template <bool FINE, int ACT>
 __device__ __forceinline__ float act_of(float z) {
     if constexpr (ACT == TB_HIP_ACT_SILU) return z * sigmoid_of<FINE>(z);
-    if constexpr (ACT == TB_HIP_ACT_GELU)
-        return 0.5f * z * (1.0f + erff(z * 0.70710678118654752440f));
+    if constexpr (ACT == TB_HIP_ACT_GELU) return z * normal_of<FINE>(z).below;
     return z;
 }
 
@@ -84,9 +113,10 @@ __device__ __forceinline__ float act_slope(float z) {
         const float s = sigmoid_of<FINE>(z);
         return fmaf(z, fmaf(-s, s, s), s);
     }
-    if constexpr (ACT == TB_HIP_ACT_GELU)
-        return 0.5f * (1.0f + erff(z * 0.70710678118654752440f)) +
-               z * (0.39894228040143267794f * exp_of<FINE>(-0.5f * z * z));
+    if constexpr (ACT == TB_HIP_ACT_GELU) {
+        const Normal n = normal_of<FINE>(z);
+        return fmaf(z, 0.39894228040143267794f * n.bell, n.below);
+    }
     return 1.0f;
 }
 
