@@ -170,8 +170,8 @@ int tb_hip_mx4_values_device(const void *codes, const void *scales, void *values
  * and at most m.  out [m, n] is dense.
  * Returns 0 for other NULL pointers, m, n, k or a_rows 0 or above 0x7fffffff,
  * experts outside 1..TB_HIP_ROUTE_MAX_EXPERTS or above 1 without offsets,
- * experts * n above 0x7fffffff, rows NULL with m other than a_rows, an
- * unknown act or dtype, or misaligned pointers. */
+ * experts * n above 0x7fffffff, m * n above 2^38, rows NULL with m other than
+ * a_rows, an unknown act or dtype, or misaligned pointers. */
 int tb_hip_mx4_product_device(const void *a_codes, const void *a_scales, size_t a_rows,
                               const int *rows, const void *w_codes, const void *w_scales,
                               const int *offsets, const float *bias, const float *row_scale,

@@ -20,7 +20,7 @@ typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
-constexpr size_t kMaxCount = 0x7fffffffu;
+constexpr size_t kMaxCount = 0x7fffffffu, kMaxOutputs = size_t(1) << 38;
 constexpr size_t kMaxGrid = 1 << 20;
 constexpr int kBlock = 32, kPad = 128;
 
@@ -253,10 +253,11 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_kernel(ProductArgs a) {
     __shared__ f32x4 sums[kFewWaves][MT][64];
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     const int low = lane & 15, part = lane >> 4;
-    const unsigned columns = (unsigned)((a.n + 15) / 16), tile = blockIdx.x / columns;
+    const unsigned block = blockIdx.y * gridDim.x + blockIdx.x;
+    const unsigned columns = (unsigned)((a.n + 15) / 16), tile = block / columns;
     RowTile rt;
     if (!find_rows(a, tile, 16 * MT, rt)) return;
-    const size_t n0 = (size_t)(blockIdx.x - tile * columns) * 16;
+    const size_t n0 = (size_t)(block - tile * columns) * 16;
     const bool some = rt.expert < a.experts;
     const size_t code_row = a.kp / 2, scale_row = a.kp / kBlock;
     const size_t wr = (n0 + low < a.n ? n0 + low : a.n - 1) + (some ? rt.expert * a.n : 0);
@@ -646,6 +647,12 @@ size_t tiles_of(const ProductArgs &a, int shape) {
     return high * ((a.n + t.columns - 1) / t.columns);
 }
 
+// A dimension of a grid holds less than 2^32 threads, 512 to a tile.  More than
+// 2^22 tiles of few rows take rows of 2^22 workgroups, the last of which find
+// no tile; staged tiles leave narrow products of 2^23 tiles and more to them.
+constexpr unsigned kGridRow = 1 << 22;
+static_assert(64 * kFewWaves * (size_t)kGridRow < size_t(1) << 32);
+
 // Measured (us; large / middle / few rows with 4, 2 and 1 row tiles; bf16 out):
 //   m 16,384 n 4,096 k 4,096: 189 / 254 / 2,230 / 2,677 / -
 //   m  8,192 n 2,048 k 1,024: 18.3 / 21.8 / 191 / 199 / 238     (256 large tiles)
@@ -665,7 +672,8 @@ int shape_for(const ProductArgs &a) {
     // The staged kernels address a matrix with 32 bits from a tile's first row
     // (from the first of all where rows are gathered) and read whole slices.
     const size_t code_row = a.kp / 2, reach = 0xffffffffu / code_row;
-    const bool staged = a.kp >= kSlice && reach >= 256 && (!a.rows || a.a_rows <= reach);
+    const bool staged = a.kp >= kSlice && reach >= 256 && (!a.rows || a.a_rows <= reach) &&
+                        tiles_of(a, kMiddle) < 2 * kGridRow;
     const size_t per = a.m / a.experts;
     if (staged && per > 32 && a.m * a.n > (1 << 18)) {
         // Half of the runs of rows end within a tile of their own, about.
@@ -683,12 +691,14 @@ int shape_for(const ProductArgs &a) {
 
 template <class T>
 void launch_product(const ProductArgs &a, int shape, unsigned tiles, hipStream_t q) {
+    const dim3 few = tiles < kGridRow ? dim3(tiles)
+                                      : dim3(kGridRow, (tiles + kGridRow - 1) / kGridRow);
     with_act(a.act, [&](auto act) {
         constexpr int ACT = decltype(act)::value;
         switch (shape) {
-            case kFew1: few_kernel<T, ACT, 1><<<tiles, 64 * kFewWaves, 0, q>>>(a); break;
-            case kFew2: few_kernel<T, ACT, 2><<<tiles, 64 * kFewWaves, 0, q>>>(a); break;
-            case kFew4: few_kernel<T, ACT, 4><<<tiles, 64 * kFewWaves, 0, q>>>(a); break;
+            case kFew1: few_kernel<T, ACT, 1><<<few, 64 * kFewWaves, 0, q>>>(a); break;
+            case kFew2: few_kernel<T, ACT, 2><<<few, 64 * kFewWaves, 0, q>>>(a); break;
+            case kFew4: few_kernel<T, ACT, 4><<<few, 64 * kFewWaves, 0, q>>>(a); break;
             case kMiddle: tile_kernel<T, ACT, 2, 2, 4, 4><<<tiles, 256, 0, q>>>(a); break;
             default: tile_kernel<T, ACT, 2, 4, 8, 4><<<tiles, 512, 0, q>>>(a); break;
         }
@@ -767,7 +777,8 @@ extern "C" int tb_hip_mx4_product_device(const void *a_codes, const void *a_scal
     if (!a_codes || !a_scales || !w_codes || !w_scales || !out || !a_rows ||
         a_rows > kMaxCount || !m || m > kMaxCount || !n || n > kMaxCount || !k ||
         k > kMaxCount || experts < 1 || experts > TB_HIP_ROUTE_MAX_EXPERTS ||
-        (experts > 1 && !offsets) || n > kMaxCount / experts || (!rows && m != a_rows) ||
+        (experts > 1 && !offsets) || n > kMaxCount / experts || m > kMaxOutputs / n ||
+        (!rows && m != a_rows) ||
         !known_act(act) || !known_type(dtype) || !multiple_of(a_codes, 16) ||
         !multiple_of(w_codes, 16) || !multiple_of(a_scales, 4) || !multiple_of(w_scales, 4) ||
         !multiple_of(out, type_size(dtype)))
@@ -792,8 +803,8 @@ extern "C" int tb_hip_mx4_product_device(const void *a_codes, const void *a_scal
     hipStream_t q = reinterpret_cast<hipStream_t>(stream);
     (void)hipGetLastError();
     const int shape = shape_for(a);
+    // Below 2^31: 2^30 for 2^38 values in tiles of 16 x 16, and the runs' ends.
     const size_t tiles = tiles_of(a, shape);
-    if (tiles > kMaxCount) return 0;
     if (dtype == TB_HIP_F32)
         launch_product<float>(a, shape, (unsigned)tiles, q);
     else if (dtype == TB_HIP_BF16)
