@@ -96,7 +96,9 @@ size_t tb_hip_group_norm_workspace_bytes(size_t images, size_t pixels, int chann
  * An expert whose logit or key is -inf is never chosen; where too few are
  * left the remaining experts are -1 and their weights 0, and so is the whole
  * row of a token whose `valid` byte (nullable, [tokens]) is 0, whose logits
- * are not read.  NaN keys count as the highest and give NaN weights.
+ * are not read.  NaN keys count as the highest.  An expert with a NaN logit has
+ * a NaN weight, with softmax or renormalise the whole row; a NaN in the bias
+ * chooses, and does not weigh either.
  * experts [tokens, k] int32, weights [tokens, k] fp32.
  * Returns 0 for NULL logits, experts or weights, tokens 0 or tokens * k above
  * 0x7fffffff, n_experts outside 1..TB_HIP_ROUTE_MAX_EXPERTS, k outside
