@@ -154,7 +154,8 @@ int tb_hip_mx4_quantise_device(const void *x, size_t row_stride, void *codes, vo
                                size_t rows, size_t k, int dtype, void *stream);
 
 /* The values [rows, k] (dense) that codes and scales stand for, rounded to
- * the type (only f16 can round or overflow).
+ * the type: f16 can round or overflow, f32 and bf16 can overflow for scales of
+ * 253 and 254, which quantisation does not give.
  * Both return 0 for NULL pointers, rows or k 0 or above 0x7fffffff, an
  * unknown dtype or misaligned pointers or stride. */
 int tb_hip_mx4_values_device(const void *codes, const void *scales, void *values, size_t rows,
