@@ -263,7 +263,10 @@ __global__ __launch_bounds__(kThreads) void route_kernel(RouteArgs given) {
                 case 1: keep_groups<Q, 1>(a, e0, lane, stands, key); break;
                 case 2: keep_groups<Q, 2>(a, e0, lane, stands, key); break;
                 case 3: keep_groups<Q, 3>(a, e0, lane, stands, key); break;
-                default: keep_groups<Q, Q == 8 ? 3 : 4>(a, e0, lane, stands, key);
+                // At eight a lane there are 16 experts at most, in groups of
+                // no more than eight.
+                default:
+                    if constexpr (Q == 16) keep_groups<Q, 4>(a, e0, lane, stands, key);
             }
         }
         if constexpr (GROUPS == kUneven) {
