@@ -9,8 +9,9 @@ which an actor over this library's sensor planes uses them.
   experts         4-bit weights: up with SiLU, down with the routing weight
   sum             token + its experts' rows
 
-The weights are random.  Buffers and workspaces are made once for a batch; an
-acting step only launches, on the current stream.
+The weights are random.  The entries' buffers and workspaces are made once for a
+batch; an acting step only launches, on the current stream.  What torch computes
+between them (patches, planes, logits, the rows' sums) it allocates itself.
 
     python examples/routed_tokens.py [environments]
 """

@@ -526,7 +526,7 @@ __global__ __launch_bounds__(kMaxThreads) void grad_apply_kernel(NormArgs a) {
 // Every thread holds NV vectors; the means, then the squared deviations, then
 // the elements come from them.  4,096 x 1,024 x 64 bf16 with SiLU: 250 us, 4.3
 // TB/s of x and y, where a copy of 4 GiB moves 4.8; 257 x 1,023 x 48 fp32 with
-// GELU: 28.6 us, 3.5 TB/s, 771 workgroups on 256 CUs.
+// GELU: 26.5 us, 3.8 TB/s, 771 workgroups on 256 CUs.
 template <class T, int B, int NV, int ACT>
 __global__ __launch_bounds__(kMaxThreads) void norm_whole_kernel(NormArgs a) {
     typedef Vec<T, B> X;

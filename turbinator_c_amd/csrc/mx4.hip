@@ -28,8 +28,10 @@ __host__ __device__ inline size_t padded(size_t k) { return (k + kPad - 1) / kPa
 
 // --------------------------------------------------------------------------
 // Quantisation: four lanes to a block of 32, eight values each, one vector in
-// and one word out.  Bound by memory: 40,960 x 2,000 bf16 44 us, the values back 37
-// us (4.7 and 5.6 TB/s of what they read and write).
+// and one word out.  Bound by memory where rows start on 16 bytes: 40,960 x
+// 2,000 bf16 44 us, the values back 37 us (4.7 and 5.6 TB/s of what they read
+// and write).  Other rows go by single elements: k 2,002 takes 2.3 and 2.7
+// times as long (89 and 104 us for 38 and 39, in a row on the same rows).
 
 constexpr int kQuantThreads = 256;
 
@@ -326,10 +328,17 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_kernel(ProductArgs a) {
 // of slice s + 1; barrier: all waves have them, and have read slice s; load
 // slice s + 2 over it, and read step 0 of slice s + 1 while multiplying step 1.
 //
-// m 16,384, n 4,096, k 4,096: 178 to 189 us, 2.9 to 3.1 PFLOP/s, half of what
+// m 16,384, n 4,096, k 4,096: 168 to 176 us, 3.1 to 3.3 PFLOP/s, half of what
 // the instruction does from registers on such values (6.4): the waves of a CU
 // meet at a barrier every 64 matrix instructions.  At short k the ends count: k
-// 1,024 takes 18.3 us for 8,192 x 2,048, of which 8 are starting and storing.
+// 1,024 takes 18.1 us for 8,192 x 2,048, of which 8 are starting and storing.
+// Outputs whose rows are off 16 bytes leave by single elements: n 4,095 takes
+// 223 us, and with k 256 114 us where n 4,096 takes 48.
+//
+// With experts the grid holds tiles for the runs' ends that may not be there,
+// the last ones of each band of columns, which the contiguous order gives to
+// some of the XCDs: 8,200 rows of 8 experts leave 94 tiles to two of them and
+// 150 to the others.
 constexpr int kSlice = 2 * kPad, kSliceBytes = kSlice / 2;
 
 typedef const __attribute__((address_space(1))) void *GlobalPtr;
@@ -654,20 +663,32 @@ constexpr unsigned kGridRow = 1 << 22;
 static_assert(64 * kFewWaves * (size_t)kGridRow < size_t(1) << 32);
 
 // Measured (us; large / middle / few rows with 4, 2 and 1 row tiles; bf16 out):
-//   m 16,384 n 4,096 k 4,096: 189 / 254 / 2,230 / 2,677 / -
-//   m  8,192 n 2,048 k 1,024: 18.3 / 21.8 / 191 / 199 / 238     (256 large tiles)
-//   m 16,384 n   512 k   512: 12.6 / 10.1 / 56 / 56 / 71        (128 large tiles)
-//   m    320 n 2,048 k 2,048: 18.1 / 10.7 / 18.0 / 17.0 / 21.4
-//   m    128 n 4,096 k 4,096: 27.9 / 17.1 / 21.3 / 24.6 / 31.7
-//   m     64 n 4,096 k 4,096: 27.4 / 16.3 / 12.4 / 13.8 / 17.5
-//   m     64 n 1,024 k 1,024: 12.1 / 7.3 / 5.6 / 4.5 / 3.9
+//   m 16,384 n 4,096 k 4,096: 168 / 210 / 2,210 / 2,650 / 3,537
+//   m  8,192 n 2,048 k 2,048: 25.5 / 36.2 / 283 / 340 / 447     (256 large tiles)
+//   m  8,192 n 2,048 k 1,024: 18.1 / 23.9 / 185 / 193 / 227
+//   m  8,192 n 2,048 k   512: 14.7 / 17.1 / 99 / 99 / 131
+//   m  8,192 n 2,048 k   256: 15.3 / 17.1 / 78 / 82 / 119
+//   m  8,200 n 2,048 k 1,024: 28.5 / 25.5 / 186 / 193 / 228
+//   m 16,384 n   512 k   512: 12.0 / 9.4 / 55 / 55 / 69         (128 large tiles)
+//   m    320 n 2,048 k 2,048: 18.0 / 10.5 / 17.7 / 16.5 / 20.7
+//   m    128 n 4,096 k 4,096: 27.8 / 16.9 / 21.5 / 24.5 / 30.9
+//   m     64 n 4,096 k 4,096: 27.2 / 16.1 / 12.4 / 13.8 / 17.2
+//   m     64 n 1,024 k 1,024: 12.0 / 7.3 / 5.6 / 4.5 / 3.9
 //   m     10 n 2,048 k 2,048: 16.8 / 9.8 / 5.3 / 4.8 / 4.4
 // So: staged tiles where the output has more than 2^18 values (a lone staged
 // tile takes about 0.7 us for 256 values of k, the few-row kernel about 3 ns
 // for a thousand outputs) and experts fill more than a quarter of a middle
 // tile; large ones, one to a CU, or middle ones, two to a CU, by what a round
-// of them takes, 8.2 + 2.4 and 3.9 + 1.8 us for each slice of k (from the
-// lines above).  Else as many row tiles as leave a workgroup to every CU.
+// of them is taken to cost, 8.2 + 2.4 and 3.9 + 1.8 us for each slice of k.
+// That is within a tenth where a round or two of k 1,024 and 2,048 run, a
+// third too little at k 256 and an eighth to a quarter too much at 16 slices
+// and many rounds, on both sides alike: the faster one is chosen in every line
+// above.  Else as many row tiles as leave a workgroup to every CU.
+//
+// What no staged tile takes goes to the few-row kernel at any size: k up to 128
+// (16,384 x 4,096: 239 us, where k 256 takes 48; 4,096 x 1,024: 18.4 and 7.6)
+// and gathered rows out of more than 4 GiB of codes (16,384 x 4,096 x 4,096:
+// 2,233 us, 176 out of less).
 int shape_for(const ProductArgs &a) {
     // The staged kernels address a matrix with 32 bits from a tile's first row
     // (from the first of all where rows are gathered) and read whole slices.
