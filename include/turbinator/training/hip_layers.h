@@ -6,8 +6,13 @@
  *     backward (the convolution stems);
  *   - routing of tokens to experts, forward and backward, and the order of
  *     the choices by expert;
+ *   - the tokens' way to their experts' rows and back, with the routing's
+ *     weights, forward and backward;
+ *   - embeddings: lookup with scaling, the order of the tokens by entry, and
+ *     the table's gradient in that order;
  *   - microscaled 4-bit floating point: quantisation, its values, and
- *     products on the scaled matrix instructions, dense or per expert.
+ *     products on the scaled matrix instructions, dense or per expert;
+ *   - rows in 8-bit integers with a scale each: the same three.
  * All pointers are device pointers.  All entries are asynchronous on `stream`
  * (a hipStream_t as void*, NULL = null stream), allocate nothing and return 1
  * iff the launches were accepted, 0 on invalid arguments (nothing is launched
@@ -35,7 +40,9 @@ enum {
     TB_HIP_NORM_MAX_CHANNELS = 65536,
     TB_HIP_ROUTE_MAX_EXPERTS = 1024,
     TB_HIP_ROUTE_MAX_K = 32,
-    TB_HIP_MX4_BLOCK = 32          /* values that share a scale */
+    TB_HIP_MX4_BLOCK = 32,         /* values that share a scale */
+    TB_HIP_EMBED_MAX_ENTRIES = 1048576,
+    TB_HIP_INT8_MAX_K = 131072     /* 127 * 127 of them fit 32 bits */
 };
 
 /* y = act((x - mean) rstd gamma + beta) over channels-last planes: `images`
@@ -139,6 +146,90 @@ int tb_hip_expert_order_device(const int *experts, const float *weights, int *of
                                void *stream);
 size_t tb_hip_expert_order_workspace_bytes(size_t tokens, int n_experts, int k);
 
+/* Tokens to their experts and back, along what tb_hip_expert_order_device
+ * gives: choice (t, j) of the tokens * k has row p = positions[t, j] of the
+ * tokens * k rows, or none (a position outside them), and weight w[t, j]
+ * (weights [tokens, k] fp32, NULL for 1).  x, out and their gradients hold
+ * `tokens` rows of `width` values, rows and their gradients tokens * k; inputs
+ * are strided (a stride may be 0), outputs dense, all of one type, at any
+ * element.  Sums run over j in order, in 32 bits, and are rounded once.
+ *
+ * rows[p] = w x[t]; the rows from offsets[n_experts] on are 0, and a choice
+ * whose position lies there has none.  Without weights rows are copied as they
+ * are.  Two choices must not have the same row. */
+int tb_hip_expert_rows_device(const void *x, size_t row_stride, const int *offsets,
+                              const int *positions, const float *weights, void *rows,
+                              size_t tokens, int n_experts, int k, size_t width, int dtype,
+                              void *stream);
+
+/* Its gradients: dx[t] = sum_j w drows[p], and, unless dweights is NULL,
+ * dweights[t, j] = the product of x[t] and drows[p] ([tokens, k] fp32; 0 for a
+ * choice without a row).  x is read for dweights only. */
+int tb_hip_expert_rows_backward_device(const void *drows, size_t drow_stride, const void *x,
+                                       size_t row_stride, const int *positions,
+                                       const float *weights, void *dx, float *dweights,
+                                       size_t tokens, int k, size_t width, int dtype,
+                                       void *stream);
+
+/* out[t] = residual[t] + sum_j w rows[p]; residual may be NULL (0).  A token
+ * without rows gets its residual. */
+int tb_hip_expert_sum_device(const void *rows, size_t row_stride, const int *positions,
+                             const float *weights, const void *residual, size_t residual_stride,
+                             void *out, size_t tokens, int k, size_t width, int dtype,
+                             void *stream);
+
+/* Its gradients: drows[p] = w dout[t], 0 from offsets[n_experts] on as above,
+ * and, unless dweights is NULL, dweights[t, j] = the product of rows[p] and
+ * dout[t].  rows is read for dweights only.  The residual's gradient is dout.
+ *
+ * The four return 0 for NULL pointers that are not said to be nullable, tokens
+ * 0 or tokens * k above 0x7fffffff, n_experts outside
+ * 1..TB_HIP_ROUTE_MAX_EXPERTS, k outside 1..TB_HIP_ROUTE_MAX_K, width 0 or
+ * above 0x7fffffff, an unknown dtype, pointers or strides off the element's
+ * size. */
+int tb_hip_expert_sum_backward_device(const void *dout, size_t dout_stride, const void *rows,
+                                      size_t row_stride, const int *offsets,
+                                      const int *positions, const float *weights, void *drows,
+                                      float *dweights, size_t tokens, int n_experts, int k,
+                                      size_t width, int dtype, void *stream);
+
+/* Embedding: out[t] = base[t] + scale table[ids[t]], `tokens` rows of `width`
+ * values from a table of `entries` rows, one rounding.  A token whose id lies
+ * outside 0..entries-1 gets its base, or 0 without one (base NULL).  table and
+ * base are strided (a stride may be 0), out is dense.
+ * Returns 0 for other NULL pointers, tokens 0 or above 0x7fffffff, entries
+ * outside 1..TB_HIP_EMBED_MAX_ENTRIES, width 0 or above 0x7fffffff, an unknown
+ * dtype, pointers or strides off the element's size. */
+int tb_hip_embed_device(const int *ids, const void *table, size_t table_stride, const void *base,
+                        size_t base_stride, float scale, void *out, size_t tokens,
+                        size_t entries, size_t width, int dtype, void *stream);
+
+/* The tokens in the order of their ids, equal ids in the order of the tokens:
+ *   order [tokens]       the token of each place, -1 behind the last entry's
+ *                        (ids outside 0..entries-1)
+ *   ranges [entries, 2]  entry v's tokens are at the places ranges[v, 0] ..
+ *                        ranges[v, 1] - 1; both 0 for an entry without tokens
+ * One order serves every gradient of these ids.  ranges must be 8-byte aligned.
+ * workspace: tb_hip_embed_order_workspace_bytes(...) bytes, 16-byte aligned.
+ * Returns 0 for NULL pointers, sizes as above, misaligned ranges or workspace. */
+int tb_hip_embed_order_device(const int *ids, int *order, int *ranges, void *workspace,
+                              size_t tokens, size_t entries, void *stream);
+size_t tb_hip_embed_order_workspace_bytes(size_t tokens, size_t entries);
+
+/* dtable[v] = scale * the sum of dout[t] over the tokens with ids[t] = v, in
+ * the order's order and in 32 bits ([entries, width] fp32, dense; rows of
+ * entries without tokens are 0).  dout is strided (the stride may be 0); rows
+ * of tokens without an entry are not read.  order and ranges as
+ * tb_hip_embed_order_device gives them for these ids.
+ * workspace: tb_hip_embed_backward_workspace_bytes(...) bytes, 16-byte aligned;
+ * it may be the order's, which is done with.
+ * Returns 0 as the two above. */
+int tb_hip_embed_backward_device(const void *dout, size_t dout_stride, const int *ids,
+                                 const int *order, const int *ranges, float scale, float *dtable,
+                                 void *workspace, size_t tokens, size_t entries, size_t width,
+                                 int dtype, void *stream);
+size_t tb_hip_embed_backward_workspace_bytes(size_t tokens, size_t entries, size_t width);
+
 /* Microscaled 4-bit floating point (the OCP MX format MXFP4): 32 consecutive
  * values of a row share a scale 2^(s - 127), s one byte, and are held as sign,
  * two exponent bits and one mantissa bit (0, 0.5, 1, 1.5, 2, 3, 4, 6).  A row
@@ -180,6 +271,37 @@ int tb_hip_mx4_product_device(const void *a_codes, const void *a_scales, size_t 
                               const int *offsets, const float *bias, const float *row_scale,
                               void *out, size_t m, size_t n, size_t k, int experts, int act,
                               int dtype, void *stream);
+
+/* Rows in 8-bit integers: code c of a row stands for c times the row's scale
+ * (fp32).  A row of k values is padded with zeros to kp = tb_hip_int8_padded(k),
+ * whole 128s: codes [rows, kp] signed bytes, scales [rows].  codes must be
+ * 16-byte, scales 4-byte aligned.
+ *
+ * Quantisation: scale = max(largest magnitude / 127, 2^-126), codes x (1 /
+ * scale) to the nearest integer, ties to even, every step before in fp32; codes
+ * lie in -127..127.  A row that holds an Inf or a NaN has the scale NaN and
+ * zero codes. */
+size_t tb_hip_int8_padded(size_t k);
+int tb_hip_int8_quantise_device(const void *x, size_t row_stride, void *codes, float *scales,
+                                size_t rows, size_t k, int dtype, void *stream);
+
+/* The values [rows, k] (dense) that codes and scales stand for, rounded to
+ * fp32 and to the type (f16 can overflow).
+ * Both return 0 for NULL pointers, rows 0 or above 0x7fffffff, k 0 or above
+ * TB_HIP_INT8_MAX_K, an unknown dtype or misaligned pointers or stride. */
+int tb_hip_int8_values_device(const void *codes, const float *scales, void *values, size_t rows,
+                              size_t k, int dtype, void *stream);
+
+/* out[r] = act(A[a(r)] W[x(r)]^T + bias[x(r)]) row_scale[r] of quantised rows:
+ * the sums of codes in 32-bit integers (exact for codes of quantisation), times
+ * A's scale, then W's, in fp32.  Arguments and refusals as tb_hip_mx4_product_device,
+ * with a_scales [a_rows] and w_scales [experts, n] and k at most
+ * TB_HIP_INT8_MAX_K.  The bytes of codes behind k must be 0 on one side. */
+int tb_hip_int8_product_device(const void *a_codes, const float *a_scales, size_t a_rows,
+                               const int *rows, const void *w_codes, const float *w_scales,
+                               const int *offsets, const float *bias, const float *row_scale,
+                               void *out, size_t m, size_t n, size_t k, int experts, int act,
+                               int dtype, void *stream);
 
 #ifdef __cplusplus
 }

@@ -13,6 +13,7 @@ import os
 import shutil
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -38,7 +39,7 @@ C_FLAGS = ["-O2", "-std=c11", "-fPIC", "-Wall", "-Wextra", "-D__HIP_PLATFORM_AMD
            f"-I{ROCM / 'include'}", f"-I{INCLUDE}"]
 
 HIP_SOURCES = ["features.hip", "onboard.hip", "sac_actor.hip", "group_norm.hip", "route.hip",
-               "mx4.hip"]
+               "mx4.hip", "expert_rows.hip", "embed.hip", "int8.hip"]
 HOST_C_SOURCES = ["feature_batch.c", "feature_pipeline.c", "sac_host.c"]
 
 LIB_HIP = PKG / "libturbinator_hip.so"
@@ -78,11 +79,11 @@ def generate_ray_table() -> Path:
 def build_hip_library() -> Path:
     BUILD.mkdir(exist_ok=True)
     generate_ray_table()
-    objs = []
-    for src in HIP_SOURCES:
-        obj = BUILD / (Path(src).stem + ".hip.o")
-        _run([hipcc(), *HIP_FLAGS, f"-I{BUILD}", "-c", str(CSRC / src), "-o", str(obj)])
-        objs.append(obj)
+    objs = [BUILD / (Path(src).stem + ".hip.o") for src in HIP_SOURCES]
+    with ThreadPoolExecutor(min(8, os.cpu_count() or 1)) as pool:
+        list(pool.map(lambda src, obj: _run([hipcc(), *HIP_FLAGS, f"-I{BUILD}", "-c",
+                                             str(CSRC / src), "-o", str(obj)]),
+                      HIP_SOURCES, objs))
     for src in HOST_C_SOURCES:
         obj = BUILD / (Path(src).stem + ".c.o")
         _run(["gcc", *C_FLAGS, "-c", str(CSRC / src), "-o", str(obj)])

@@ -1,0 +1,638 @@
+// Embeddings (hip_layers.h): lookup with scaling, the order of the tokens by
+// entry, and the table's gradient in that order.
+//
+//   lookup     out[t] = base[t] + scale table[id[t]]
+//   order      the tokens sorted by id, equal ids in the order of the tokens;
+//              range v = the places of entry v's tokens in it
+//   gradient   dtable[v] = scale sum_{t: id[t] = v} dout[t]
+//
+// The gradient adds rows up in the order's order, so that it never depends on
+// timing; every entry's row is written once, dout is read once.
+#include "layer_math.h"
+
+namespace {
+
+using namespace layer;
+
+typedef int i32x2 __attribute__((ext_vector_type(2)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+constexpr int kThreads = 256;
+constexpr size_t kMaxCount = 0x7fffffffu, kMaxGrid = 1 << 20;
+
+unsigned grid_of(size_t items, size_t per) {
+    const size_t want = (items + per - 1) / per;
+    return (unsigned)(want < kMaxGrid ? want : kMaxGrid);
+}
+
+// Rows in vectors of B bytes, the last of which ends with the row and repeats
+// some of the one before; `lanes` lanes, a power of two, have a vector each.
+struct RowShape {
+    unsigned width, vectors, pieces, lanes;
+};
+
+template <class T, int B>
+RowShape shape_of(size_t width) {
+    RowShape s;
+    s.width = (unsigned)width;
+    s.vectors = (unsigned)((width * sizeof(T) + B - 1) / B);
+    s.pieces = (s.vectors + 63) / 64;
+    s.lanes = 1;
+    while (s.lanes < s.vectors && s.lanes < 64) s.lanes *= 2;
+    return s;
+}
+
+// Vector v's first element.
+template <int N>
+__device__ __forceinline__ unsigned first_of(const RowShape &s, unsigned v) {
+    return (v + 1) * N <= s.width ? v * N : s.width - N;
+}
+
+// --------------------------------------------------------------------------
+// Lookup
+
+struct LookupArgs {
+    const int *ids;
+    const char *table, *base;
+    char *out;
+    size_t table_stride, base_stride, tokens, entries;
+    float scale;
+    RowShape s;
+};
+
+template <class T, int B, int LANES>
+__global__ __launch_bounds__(kThreads) void lookup_kernel(LookupArgs a) {
+    typedef Vec<T, B> X;
+    typedef typename X::raw raw;
+    const unsigned lanes = LANES ? LANES : a.s.lanes, lane = threadIdx.x & (lanes - 1);
+    const unsigned groups = kThreads / lanes;
+    unsigned group = threadIdx.x / lanes;
+    if (LANES == 64) group = __builtin_amdgcn_readfirstlane(group);
+    const size_t items = a.tokens * a.s.pieces, row_bytes = (size_t)a.s.width * sizeof(T);
+    for (size_t item = (size_t)blockIdx.x * groups + group; item < items;
+         item += (size_t)gridDim.x * groups) {
+        const size_t t = a.s.pieces > 1 ? item / a.s.pieces : item;
+        const unsigned v = (unsigned)(item - t * a.s.pieces) * lanes + lane;
+        if (v >= a.s.vectors) continue;
+        const unsigned e = first_of<X::n>(a.s, v);
+        const int id = a.ids[t];
+        raw out = {};
+        if (a.base) out = load_loose<T, B>(a.base + t * a.base_stride, e);
+        if (id >= 0 && (size_t)id < a.entries) {
+            float x[X::n], y[X::n];
+            X::unpack(load_loose<T, B>(a.table + (size_t)id * a.table_stride, e), x);
+            X::unpack(out, y);
+#pragma unroll
+            for (int i = 0; i < X::n; ++i)
+                y[i] = a.base ? fmaf(a.scale, x[i], y[i]) : a.scale * x[i];
+            out = X::pack(y);
+        }
+        store_loose<T, B>(a.out + t * row_bytes, e, out);
+    }
+}
+
+// --------------------------------------------------------------------------
+// Order
+
+struct OrderArgs {
+    const int *ids, *from;  // from: the order of the pass before, NULL for none
+    int *to;
+    i32x2 *ranges;
+    int *counts;            // [segments][digits + 1]
+    size_t tokens, entries, segment;
+    unsigned segments;
+    int shift, bits, last;
+};
+
+// The entry of a token, `entries` for none.
+__device__ __forceinline__ unsigned entry_of(const int *ids, size_t entries, size_t t) {
+    const unsigned id = (unsigned)ids[t];
+    return id < entries ? id : (unsigned)entries;
+}
+
+__global__ __launch_bounds__(kThreads) void clear_kernel(i32x2 *ranges, size_t entries) {
+    for (size_t v = (size_t)blockIdx.x * kThreads + threadIdx.x; v < entries;
+         v += (size_t)gridDim.x * kThreads)
+        ranges[v] = (i32x2){0, 0};
+}
+
+// Few tokens: a token's place is the number of smaller keys and of equal ones
+// before it.  Each lane has a token, each wave a share of the keys, which come
+// through scalar loads; the shares are added up in LDS.
+constexpr int kRankWaves = 16;
+constexpr size_t kRankMost = 4096;
+
+__global__ __launch_bounds__(64 * kRankWaves) void rank_kernel(OrderArgs a) {
+    __shared__ int parts[kRankWaves][3][64];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int n = (int)a.tokens, i0 = blockIdx.x * 64, i = i0 + lane;
+    const unsigned key = i < n ? entry_of(a.ids, a.entries, i) : 0;
+    const int per = (n + kRankWaves - 1) / kRankWaves;
+    const int j0 = wave * per, j1 = j0 + per < n ? j0 + per : n;
+    int less = 0, most = 0, place = 0;  // smaller keys, those and equal ones, keys in front
+    const int a0 = j1 < i0 ? j1 : i0;
+    for (int j = j0; j < a0; ++j) {
+        const unsigned o = entry_of(a.ids, a.entries, j);
+        less += o < key;
+        most += o <= key;
+    }
+    place = most;
+    const int b1 = j1 < i0 + 64 ? j1 : i0 + 64;
+    for (int j = j0 > i0 ? j0 : i0; j < b1; ++j) {
+        const unsigned o = entry_of(a.ids, a.entries, j);
+        less += o < key;
+        most += o <= key;
+        place += o < key || (o == key && j < i);
+    }
+    const int before = less;
+    for (int j = j0 > i0 + 64 ? j0 : i0 + 64; j < j1; ++j) {
+        const unsigned o = entry_of(a.ids, a.entries, j);
+        less += o < key;
+        most += o <= key;
+    }
+    place += less - before;
+    parts[wave][0][lane] = less;
+    parts[wave][1][lane] = most;
+    parts[wave][2][lane] = place;
+    __syncthreads();
+    if (wave || i >= n) return;
+    for (int w = 1; w < kRankWaves; ++w) {
+        less += parts[w][0][lane];
+        most += parts[w][1][lane];
+        place += parts[w][2][lane];
+    }
+    const bool known = key < a.entries;
+    a.to[place] = known ? i : -1;
+    if (known && place == less) a.ranges[key] = (i32x2){less, most};
+}
+
+// Many tokens: a stable counting sort by digits, the least first; tokens
+// without an entry have a digit of their own behind the others.  A workgroup
+// has a segment of the tokens, each of its waves a run of it.
+constexpr int kSortWaves = 8, kSortThreads = 64 * kSortWaves;
+constexpr size_t kSegment = 2048, kMaxSegments = 256;
+
+__device__ __forceinline__ unsigned digit_of(const OrderArgs &a, size_t c, int &token) {
+    token = a.from ? a.from[c] : (int)c;
+    const unsigned id = (unsigned)a.ids[token];
+    return id < a.entries ? id >> a.shift & ((1u << a.bits) - 1) : 1u << a.bits;
+}
+
+__global__ __launch_bounds__(kSortThreads) void count_kernel(OrderArgs a) {
+    extern __shared__ int lds[];
+    const int digits = (1 << a.bits) + 1;
+    for (int d = threadIdx.x; d < digits; d += kSortThreads) lds[d] = 0;
+    __syncthreads();
+    const size_t c0 = blockIdx.x * a.segment;
+    const size_t c1 = c0 + a.segment < a.tokens ? c0 + a.segment : a.tokens;
+    for (size_t c = c0 + threadIdx.x; c < c1; c += kSortThreads) {
+        int token;
+        atomicAdd(&lds[digit_of(a, c, token)], 1);
+    }
+    __syncthreads();
+    for (int d = threadIdx.x; d < digits; d += kSortThreads)
+        a.counts[(size_t)blockIdx.x * digits + d] = lds[d];
+    if (!a.shift)
+        for (size_t v = (size_t)blockIdx.x * kSortThreads + threadIdx.x; v < a.entries;
+             v += (size_t)gridDim.x * kSortThreads)
+            a.ranges[v] = (i32x2){0, 0};
+}
+
+__global__ __launch_bounds__(kSortThreads) void place_kernel(OrderArgs a) {
+    extern __shared__ int lds[];
+    const int digits = (1 << a.bits) + 1, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    int *start = lds, *next = lds + digits * (1 + wave);
+    for (int i = threadIdx.x; i < digits * kSortWaves; i += kSortThreads) lds[digits + i] = 0;
+    __syncthreads();
+    const size_t run = a.segment / kSortWaves, c0 = blockIdx.x * a.segment + wave * run;
+    const size_t c1 = c0 + run < a.tokens ? c0 + run : a.tokens;
+    int token;
+    for (size_t c = c0 + lane; c < c1; c += 64) atomicAdd(&next[digit_of(a, c, token)], 1);
+    // Of each digit: all segments' counts, and those of the segments before.
+    for (int d = threadIdx.x; d < digits; d += kSortThreads) {
+        int all = 0, before = 0;
+        for (unsigned s = 0; s < a.segments; ++s) {
+            const int n = a.counts[(size_t)s * digits + d];
+            all += n;
+            before += s < blockIdx.x ? n : 0;
+        }
+        start[d] = all;
+        lds[digits * (1 + kSortWaves) + d] = before;
+    }
+    __syncthreads();
+    if (wave == 0) {
+        int below = 0;
+        for (int d0 = 0; d0 < digits; d0 += 64) {
+            const int d = d0 + lane, n = d < digits ? start[d] : 0, sum = running_sum(n);
+            if (d < digits) start[d] = below + sum - n + lds[digits * (1 + kSortWaves) + d];
+            below += __builtin_amdgcn_readlane(sum, 63);
+        }
+    }
+    __syncthreads();
+    for (int d = threadIdx.x; d < digits; d += kSortThreads) {
+        int at = start[d];
+        for (int w = 0; w < kSortWaves; ++w) {
+            const int n = lds[digits * (1 + w) + d];
+            lds[digits * (1 + w) + d] = at;
+            at += n;
+        }
+    }
+    __syncthreads();
+    for (size_t b = c0; b < c1; b += 64) {
+        const bool live = b + lane < c1;
+        unsigned d = 0;
+        if (live) d = digit_of(a, b + lane, token);
+        // The lanes with the same digit.
+        unsigned long long same = __ballot(live);
+        for (int bit = 0; bit <= a.bits; ++bit) {
+            const bool set = d >> bit & 1;
+            const unsigned long long all = __ballot(set);
+            same &= set ? all : ~all;
+        }
+        const int rank = __popcll(same & ((1ull << lane) - 1));
+        int at = 0;
+        if (live) at = next[d] + rank;
+        wave_fence();
+        if (live && rank == 0) next[d] = at + __popcll(same);
+        wave_fence();
+        if (live) a.to[at] = a.last && d == 1u << a.bits ? -1 : token;
+    }
+}
+
+// The ranges from the places where the entry changes.
+__global__ __launch_bounds__(kThreads) void range_kernel(OrderArgs a) {
+    for (size_t c = (size_t)blockIdx.x * kThreads + threadIdx.x; c < a.tokens;
+         c += (size_t)gridDim.x * kThreads) {
+        const int token = a.to[c];
+        if (token < 0) continue;
+        const int id = a.ids[token], front = c ? a.to[c - 1] : -1;
+        const int behind = c + 1 < a.tokens ? a.to[c + 1] : -1;
+        int *range = reinterpret_cast<int *>(a.ranges + id);
+        if (front < 0 || a.ids[front] != id) range[0] = (int)c;
+        if (behind < 0 || a.ids[behind] != id) range[1] = (int)c + 1;
+    }
+}
+
+// --------------------------------------------------------------------------
+// Gradient.  An entry with at most kChunk tokens is summed by one group of
+// lanes.  Longer ranges are cut where the order's chunks of kChunk places end:
+// a chunk has parts of at most two of them, the one that its first place
+// belongs to and the one that its last does; the parts are summed side by side
+// into the workspace and joined afterwards.
+
+constexpr size_t kChunk = 32;
+
+struct GradArgs {
+    const char *dout;
+    size_t stride;
+    const int *ids, *order;
+    const i32x2 *ranges;
+    float *dtable, *parts;  // parts: [chunks][2][part_width]
+    size_t tokens, entries, part_width, chunks, chunk_blocks;
+    float scale;
+    RowShape s;
+};
+
+// An entry's range, within the order whatever it holds.
+__device__ __forceinline__ i32x2 range_of(const GradArgs &a, size_t v) {
+    i32x2 r = a.ranges[v];
+    r[0] = r[0] < 0 ? 0 : r[0];
+    r[1] = (size_t)(r[1] < 0 ? 0 : r[1]) < a.tokens ? r[1] : (int)a.tokens;
+    return r;
+}
+
+// The entry of a place of the order, -1 for none.
+__device__ __forceinline__ long long entry_at(const GradArgs &a, size_t place) {
+    const int t = a.order[place];
+    if (t < 0 || (size_t)t >= a.tokens) return -1;
+    const int id = a.ids[t];
+    return id >= 0 && (size_t)id < a.entries ? id : -1;
+}
+
+// Adds up element e on of the rows at places b .. end-1 of the order.
+template <class T, int B>
+__device__ __forceinline__ void add_rows(const GradArgs &a, long long b, long long end, unsigned e,
+                                         float (&sum)[Vec<T, B>::n]) {
+    typedef Vec<T, B> X;
+    constexpr int kAhead = 8;
+    for (; b < end; b += kAhead) {
+        typename X::raw row[kAhead];
+        bool there[kAhead];
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            const int t = a.order[b + i < end ? b + i : end - 1];
+            there[i] = b + i < end && t >= 0 && (size_t)t < a.tokens;
+            if (there[i]) row[i] = load_loose<T, B>(a.dout + (size_t)t * a.stride, e);
+        }
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            if (!there[i]) continue;
+            float x[X::n];
+            X::unpack(row[i], x);
+#pragma unroll
+            for (int j = 0; j < X::n; ++j) sum[j] += x[j];
+        }
+    }
+}
+
+template <int N>
+__device__ __forceinline__ void store_floats(float *row, unsigned e, const float (&v)[N],
+                                             float scale) {
+    constexpr int kPart = N < 4 ? N : 4;
+    typedef Vec<float, kPart * 4> F;
+#pragma unroll
+    for (int p = 0; p < N; p += kPart) {
+        float part[kPart];
+#pragma unroll
+        for (int j = 0; j < kPart; ++j) part[j] = v[p + j] * scale;
+        store_loose<float, kPart * 4>(reinterpret_cast<char *>(row), e + p, F::pack(part));
+    }
+}
+
+template <class T, int B, int LANES>
+__global__ __launch_bounds__(kThreads) void grad_kernel(GradArgs a) {
+    constexpr int N = Vec<T, B>::n;
+    const unsigned lanes = LANES ? LANES : a.s.lanes, lane = threadIdx.x & (lanes - 1);
+    const unsigned groups = kThreads / lanes;
+    unsigned group = threadIdx.x / lanes;
+    if (LANES == 64) group = __builtin_amdgcn_readfirstlane(group);
+    const bool whole = blockIdx.x >= a.chunk_blocks;
+    const size_t block = whole ? blockIdx.x - a.chunk_blocks : blockIdx.x;
+    const size_t blocks = whole ? gridDim.x - a.chunk_blocks : a.chunk_blocks;
+    const size_t items = (whole ? a.entries : a.chunks) * a.s.pieces;
+    for (size_t item = block * groups + group; item < items; item += blocks * groups) {
+        const size_t at = a.s.pieces > 1 ? item / a.s.pieces : item;
+        const unsigned v = (unsigned)(item - at * a.s.pieces) * lanes + lane;
+        if (v >= a.s.vectors) continue;
+        const unsigned e = first_of<N>(a.s, v);
+        float sum[N] = {};
+        if (whole) {
+            const i32x2 r = range_of(a, at);
+            if (r[1] - r[0] > (int)kChunk) continue;
+            add_rows<T, B>(a, r[0], r[1], e, sum);
+            store_floats<N>(a.dtable + at * a.s.width, e, sum, a.scale);
+            continue;
+        }
+        const size_t c0 = at * kChunk, c1 = c0 + kChunk < a.tokens ? c0 + kChunk : a.tokens;
+        const long long head = entry_at(a, c0), tail = entry_at(a, c1 - 1);
+        float *part = a.parts + at * 2 * a.part_width;
+        if (head >= 0) {
+            const i32x2 r = range_of(a, head);
+            if (r[1] - r[0] > (int)kChunk) {
+                add_rows<T, B>(a, (long long)c0, r[1] < (long long)c1 ? r[1] : (long long)c1, e,
+                               sum);
+                store_floats<N>(part, e, sum, 1.0f);
+            }
+        }
+        if (tail >= 0 && tail != head) {
+            const i32x2 r = range_of(a, tail);
+            if (r[1] - r[0] > (int)kChunk) {
+                float other[N] = {};
+                add_rows<T, B>(a, r[0] > (long long)c0 ? r[0] : (long long)c0, (long long)c1, e,
+                               other);
+                store_floats<N>(part + a.part_width, e, other, 1.0f);
+            }
+        }
+    }
+}
+
+// Joins the parts of the long range that starts in a chunk, if one does: 64
+// columns to a workgroup, 16 lanes of four; 16 parts at a time.
+constexpr int kJoinLanes = 16, kJoinGroups = kThreads / kJoinLanes, kJoinColumns = 4 * kJoinLanes;
+
+__global__ __launch_bounds__(kThreads) void join_kernel(GradArgs a) {
+    __shared__ f32x4 sums[kJoinGroups][kJoinLanes];
+    const size_t slices = (a.s.width + kJoinColumns - 1) / kJoinColumns;
+    const unsigned lane = threadIdx.x % kJoinLanes, group = threadIdx.x / kJoinLanes;
+    for (size_t item = blockIdx.x; item < a.chunks * slices; item += gridDim.x) {
+        const size_t chunk = item / slices, c0 = chunk * kChunk;
+        const size_t c1 = c0 + kChunk < a.tokens ? c0 + kChunk : a.tokens;
+        const long long entry = entry_at(a, c1 - 1);
+        if (entry < 0) continue;
+        const i32x2 r = range_of(a, entry);
+        if (r[1] - r[0] <= (int)kChunk || (size_t)r[0] < c0 || (size_t)r[0] >= c1) continue;
+        const size_t column = (item - chunk * slices) * kJoinColumns + lane * 4;
+        const size_t last = ((size_t)r[1] - 1) / kChunk;
+        f32x4 sum = {0, 0, 0, 0};
+        if (column < a.part_width)
+#pragma unroll 4
+            for (size_t c = chunk + group; c <= last; c += kJoinGroups) {
+                const size_t slot = c == chunk && (size_t)r[0] > c0;
+                sum += *reinterpret_cast<const f32x4 *>(a.parts + (2 * c + slot) * a.part_width +
+                                                        column);
+            }
+        sums[group][lane] = sum;
+        __syncthreads();
+        if (threadIdx.x < kJoinColumns) {
+            const size_t c = (item - chunk * slices) * kJoinColumns + threadIdx.x;
+            float all = 0.0f;
+            for (int g = 0; g < kJoinGroups; ++g)
+                all += sums[g][threadIdx.x / 4][threadIdx.x % 4];
+            if (c < a.s.width) a.dtable[(size_t)entry * a.s.width + c] = all * a.scale;
+        }
+        __syncthreads();
+    }
+}
+
+// --------------------------------------------------------------------------
+
+bool sizes_ok(size_t tokens, size_t entries) {
+    return tokens && tokens <= kMaxCount && entries && entries <= TB_HIP_EMBED_MAX_ENTRIES;
+}
+
+bool rows_ok(const void *p, size_t stride, int dtype) {
+    return p && multiple_of(p, type_size(dtype)) && stride % type_size(dtype) == 0;
+}
+
+int log2_up(size_t n) {
+    int bits = 0;
+    while (size_t(1) << bits < n) ++bits;
+    return bits;
+}
+
+struct SortShape {
+    int low, high;  // bits of the digits, high 0 for a single one
+    size_t segment;
+    unsigned segments;
+};
+
+SortShape sort_shape(size_t tokens, size_t entries) {
+    SortShape s;
+    const int bits = log2_up(entries);
+    s.low = bits <= 10 ? bits : (bits + 1) / 2;
+    s.high = bits - s.low;
+    s.segment = kSegment;
+    const size_t least = (tokens + kMaxSegments - 1) / kMaxSegments;
+    if (least > s.segment) s.segment = (least + kSortThreads - 1) / kSortThreads * kSortThreads;
+    s.segments = (unsigned)((tokens + s.segment - 1) / s.segment);
+    return s;
+}
+
+size_t whole16(size_t bytes) { return (bytes + 15) & ~size_t(15); }
+size_t count_bytes(const SortShape &s) {
+    return whole16(s.segments * ((size_t(1) << s.low) + 1) * sizeof(int));
+}
+
+void sort_pass(OrderArgs &a, int shift, int bits, hipStream_t q) {
+    a.shift = shift;
+    a.bits = bits;
+    const size_t row = ((size_t(1) << bits) + 1) * sizeof(int);
+    count_kernel<<<a.segments, kSortThreads, row, q>>>(a);
+    place_kernel<<<a.segments, kSortThreads, row * (2 + kSortWaves), q>>>(a);
+}
+
+size_t chunks_of(size_t tokens) { return (tokens + kChunk - 1) / kChunk; }
+size_t part_width(size_t width) { return (width + 3) / 4 * 4; }
+
+template <class T, int B>
+void launch_lookup(LookupArgs &a, hipStream_t q) {
+    a.s = shape_of<T, B>(a.s.width);
+    const unsigned grid = grid_of(a.tokens * a.s.pieces, kThreads / a.s.lanes);
+    if constexpr (B == 16)
+        if (a.s.lanes == 64) {
+            lookup_kernel<T, B, 64><<<grid, kThreads, 0, q>>>(a);
+            return;
+        }
+    lookup_kernel<T, B, 0><<<grid, kThreads, 0, q>>>(a);
+}
+
+template <class T, int B>
+void launch_grad(GradArgs &a, hipStream_t q) {
+    a.s = shape_of<T, B>(a.s.width);
+    const size_t per = kThreads / a.s.lanes;
+    // Chunks that no range is longer than need no joining.
+    const bool join = a.tokens > kChunk;
+    a.chunk_blocks = join ? grid_of(a.chunks * a.s.pieces, per) : 0;
+    const unsigned grid = grid_of(a.entries * a.s.pieces, per) + (unsigned)a.chunk_blocks;
+    bool wide = false;
+    if constexpr (B == 16) {
+        wide = a.s.lanes == 64;
+        if (wide) grad_kernel<T, B, 64><<<grid, kThreads, 0, q>>>(a);
+    }
+    if (!wide) grad_kernel<T, B, 0><<<grid, kThreads, 0, q>>>(a);
+    if (join) {
+        const size_t slices = (a.s.width + kJoinColumns - 1) / kJoinColumns;
+        join_kernel<<<grid_of(a.chunks * slices, 1), kThreads, 0, q>>>(a);
+    }
+}
+
+// Calls f with a zero of the type and a vector's bytes: rows shorter than a
+// vector go by single elements.
+template <class F>
+void with_type(int dtype, size_t width, F f) {
+    const bool whole = width * type_size(dtype) >= 16;
+    if (dtype == TB_HIP_F32)
+        whole ? f(0.0f, Int<16>()) : f(0.0f, Int<4>());
+    else if (dtype == TB_HIP_BF16)
+        whole ? f((__bf16)0.0f, Int<16>()) : f((__bf16)0.0f, Int<2>());
+    else
+        whole ? f((_Float16)0.0f, Int<16>()) : f((_Float16)0.0f, Int<2>());
+}
+
+}  // namespace
+
+extern "C" int tb_hip_embed_device(const int *ids, const void *table, size_t table_stride,
+                                   const void *base, size_t base_stride, float scale, void *out,
+                                   size_t tokens, size_t entries, size_t width, int dtype,
+                                   void *stream) {
+    if (!ids || !sizes_ok(tokens, entries) || !width || width > kMaxCount || !known_type(dtype) ||
+        !rows_ok(table, table_stride, dtype) || !rows_ok(out, 0, dtype) ||
+        (base && !rows_ok(base, base_stride, dtype)))
+        return 0;
+    LookupArgs a = {};
+    a.ids = ids;
+    a.table = static_cast<const char *>(table);
+    a.table_stride = table_stride;
+    a.base = static_cast<const char *>(base);
+    a.base_stride = base_stride;
+    a.scale = scale;
+    a.out = static_cast<char *>(out);
+    a.tokens = tokens;
+    a.entries = entries;
+    a.s.width = (unsigned)width;
+    hipStream_t q = reinterpret_cast<hipStream_t>(stream);
+    (void)hipGetLastError();
+    with_type(dtype, width, [&](auto zero, auto bytes) {
+        launch_lookup<decltype(zero), decltype(bytes)::value>(a, q);
+    });
+    return hipGetLastError() == hipSuccess;
+}
+
+extern "C" size_t tb_hip_embed_order_workspace_bytes(size_t tokens, size_t entries) {
+    if (!sizes_ok(tokens, entries)) return 0;
+    const SortShape s = sort_shape(tokens, entries);
+    return count_bytes(s) + whole16(tokens * sizeof(int));
+}
+
+extern "C" int tb_hip_embed_order_device(const int *ids, int *order, int *ranges, void *workspace,
+                                         size_t tokens, size_t entries, void *stream) {
+    if (!ids || !order || !ranges || !multiple_of(ranges, 8) || !workspace ||
+        !multiple_of(workspace, 16) || !sizes_ok(tokens, entries))
+        return 0;
+    OrderArgs a = {};
+    a.ids = ids;
+    a.to = order;
+    a.ranges = reinterpret_cast<i32x2 *>(ranges);
+    a.tokens = tokens;
+    a.entries = entries;
+    hipStream_t q = reinterpret_cast<hipStream_t>(stream);
+    (void)hipGetLastError();
+    if (tokens <= kRankMost) {
+        clear_kernel<<<grid_of(entries, kThreads), kThreads, 0, q>>>(a.ranges, entries);
+        rank_kernel<<<(unsigned)((tokens + 63) / 64), 64 * kRankWaves, 0, q>>>(a);
+        return hipGetLastError() == hipSuccess;
+    }
+    const SortShape s = sort_shape(tokens, entries);
+    a.counts = static_cast<int *>(workspace);
+    a.segment = s.segment;
+    a.segments = s.segments;
+    if (s.high) {
+        int *half = reinterpret_cast<int *>(static_cast<char *>(workspace) + count_bytes(s));
+        a.to = half;
+        sort_pass(a, 0, s.low, q);
+        a.from = half;
+        a.to = order;
+    }
+    a.last = 1;
+    sort_pass(a, s.high ? s.low : 0, s.high ? s.high : s.low, q);
+    range_kernel<<<grid_of(tokens, kThreads), kThreads, 0, q>>>(a);
+    return hipGetLastError() == hipSuccess;
+}
+
+extern "C" size_t tb_hip_embed_backward_workspace_bytes(size_t tokens, size_t entries,
+                                                        size_t width) {
+    if (!sizes_ok(tokens, entries) || !width || width > kMaxCount) return 0;
+    return chunks_of(tokens) * 2 * part_width(width) * sizeof(float);
+}
+
+extern "C" int tb_hip_embed_backward_device(const void *dout, size_t dout_stride, const int *ids,
+                                            const int *order, const int *ranges, float scale,
+                                            float *dtable, void *workspace, size_t tokens,
+                                            size_t entries, size_t width, int dtype,
+                                            void *stream) {
+    if (!ids || !order || !ranges || !multiple_of(ranges, 8) || !dtable ||
+        !multiple_of(dtable, 4) || !workspace || !multiple_of(workspace, 16) ||
+        !sizes_ok(tokens, entries) || !width || width > kMaxCount || !known_type(dtype) ||
+        !rows_ok(dout, dout_stride, dtype))
+        return 0;
+    GradArgs a = {};
+    a.dout = static_cast<const char *>(dout);
+    a.stride = dout_stride;
+    a.ids = ids;
+    a.order = order;
+    a.ranges = reinterpret_cast<const i32x2 *>(ranges);
+    a.scale = scale;
+    a.dtable = dtable;
+    a.parts = static_cast<float *>(workspace);
+    a.tokens = tokens;
+    a.entries = entries;
+    a.part_width = part_width(width);
+    a.chunks = chunks_of(tokens);
+    a.s.width = (unsigned)width;
+    hipStream_t q = reinterpret_cast<hipStream_t>(stream);
+    (void)hipGetLastError();
+    with_type(dtype, width, [&](auto zero, auto bytes) {
+        launch_grad<decltype(zero), decltype(bytes)::value>(a, q);
+    });
+    return hipGetLastError() == hipSuccess;
+}

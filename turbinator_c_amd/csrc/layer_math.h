@@ -45,6 +45,19 @@ struct Vec {
     }
 };
 
+// B bytes of a row of T at any element: global memory takes 16-byte accesses at
+// any address, so rows of odd widths go by whole vectors too.
+template <class T, int B>
+using Loose __attribute__((aligned(sizeof(T)))) = typename Raw<B>::type;
+template <class T, int B>
+__device__ __forceinline__ typename Raw<B>::type load_loose(const char *row, size_t element) {
+    return *reinterpret_cast<const Loose<T, B> *>(row + element * sizeof(T));
+}
+template <class T, int B>
+__device__ __forceinline__ void store_loose(char *row, size_t element, typename Raw<B>::type v) {
+    *reinterpret_cast<Loose<T, B> *>(row + element * sizeof(T)) = v;
+}
+
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kLog2eLow = 1.92596299112661887e-8f;  // log2(e) - kLog2e
 constexpr float kLn2 = 0.69314718055994530942f;
@@ -129,6 +142,12 @@ __device__ __forceinline__ int running_sum(int v) {
     v += __builtin_amdgcn_update_dpp(0, v, 0x118, 15, 15, false);
     v += __builtin_amdgcn_update_dpp(0, v, 0x142, 10, 15, false);
     return v + __builtin_amdgcn_update_dpp(0, v, 0x143, 12, 15, false);
+}
+
+// LDS that only the calling wave uses: its accesses are in order.
+__device__ __forceinline__ void wave_fence() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
 }
 
 // Calls f with the activation as a compile-time constant.

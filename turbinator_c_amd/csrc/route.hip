@@ -83,12 +83,6 @@ __device__ __forceinline__ int lanes_min_int(int v, int lanes) {
     return over_lanes(v, lanes, [](int a, int b) { return a < b ? a : b; });
 }
 
-// LDS that only the calling wave uses: its accesses are in order.
-__device__ __forceinline__ void wave_fence() {
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-}
-
 template <class T>
 __device__ __forceinline__ float element(const char *row, int i) {
     return (float)reinterpret_cast<const T *>(row)[i];

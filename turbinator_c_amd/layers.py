@@ -107,7 +107,105 @@ def mx4_product_device(a_codes, a_scales, a_rows: int, rows, w_codes, w_scales, 
         _stream(stream))
 
 
+def expert_rows_device(x, row_stride: int, offsets, positions, weights, rows, tokens: int,
+                       n_experts: int, k: int, width: int, dtype: int, stream=None) -> int:
+    """tb_hip_expert_rows_device."""
+    return hip_lib().tb_hip_expert_rows_device(
+        _dev(x), row_stride, _dev(offsets), _dev(positions), _dev(weights), _dev(rows), tokens,
+        n_experts, k, width, dtype, _stream(stream))
+
+
+def expert_rows_backward_device(drows, drow_stride: int, x, row_stride: int, positions, weights,
+                                dx, dweights, tokens: int, k: int, width: int, dtype: int,
+                                stream=None) -> int:
+    """tb_hip_expert_rows_backward_device."""
+    return hip_lib().tb_hip_expert_rows_backward_device(
+        _dev(drows), drow_stride, _dev(x), row_stride, _dev(positions), _dev(weights), _dev(dx),
+        _dev(dweights), tokens, k, width, dtype, _stream(stream))
+
+
+def expert_sum_device(rows, row_stride: int, positions, weights, residual, residual_stride: int,
+                      out, tokens: int, k: int, width: int, dtype: int, stream=None) -> int:
+    """tb_hip_expert_sum_device."""
+    return hip_lib().tb_hip_expert_sum_device(
+        _dev(rows), row_stride, _dev(positions), _dev(weights), _dev(residual), residual_stride,
+        _dev(out), tokens, k, width, dtype, _stream(stream))
+
+
+def expert_sum_backward_device(dout, dout_stride: int, rows, row_stride: int, offsets, positions,
+                               weights, drows, dweights, tokens: int, n_experts: int, k: int,
+                               width: int, dtype: int, stream=None) -> int:
+    """tb_hip_expert_sum_backward_device."""
+    return hip_lib().tb_hip_expert_sum_backward_device(
+        _dev(dout), dout_stride, _dev(rows), row_stride, _dev(offsets), _dev(positions),
+        _dev(weights), _dev(drows), _dev(dweights), tokens, n_experts, k, width, dtype,
+        _stream(stream))
+
+
+def embed_device(ids, table, table_stride: int, base, base_stride: int, scale: float, out,
+                 tokens: int, entries: int, width: int, dtype: int, stream=None) -> int:
+    """tb_hip_embed_device."""
+    return hip_lib().tb_hip_embed_device(
+        _dev(ids), _dev(table), table_stride, _dev(base), base_stride, scale, _dev(out), tokens,
+        entries, width, dtype, _stream(stream))
+
+
+def embed_order_workspace_bytes(tokens: int, entries: int) -> int:
+    return hip_lib().tb_hip_embed_order_workspace_bytes(tokens, entries)
+
+
+def embed_order_device(ids, order, ranges, workspace, tokens: int, entries: int,
+                       stream=None) -> int:
+    """tb_hip_embed_order_device."""
+    return hip_lib().tb_hip_embed_order_device(_dev(ids), _dev(order), _dev(ranges),
+                                               _dev(workspace), tokens, entries, _stream(stream))
+
+
+def embed_backward_workspace_bytes(tokens: int, entries: int, width: int) -> int:
+    return hip_lib().tb_hip_embed_backward_workspace_bytes(tokens, entries, width)
+
+
+def embed_backward_device(dout, dout_stride: int, ids, order, ranges, scale: float, dtable,
+                          workspace, tokens: int, entries: int, width: int, dtype: int,
+                          stream=None) -> int:
+    """tb_hip_embed_backward_device."""
+    return hip_lib().tb_hip_embed_backward_device(
+        _dev(dout), dout_stride, _dev(ids), _dev(order), _dev(ranges), scale, _dev(dtable),
+        _dev(workspace), tokens, entries, width, dtype, _stream(stream))
+
+
+def int8_padded(k: int) -> int:
+    return hip_lib().tb_hip_int8_padded(k)
+
+
+def int8_quantise_device(x, row_stride: int, codes, scales, rows: int, k: int, dtype: int,
+                         stream=None) -> int:
+    """tb_hip_int8_quantise_device."""
+    return hip_lib().tb_hip_int8_quantise_device(_dev(x), row_stride, _dev(codes), _dev(scales),
+                                                 rows, k, dtype, _stream(stream))
+
+
+def int8_values_device(codes, scales, values, rows: int, k: int, dtype: int, stream=None) -> int:
+    """tb_hip_int8_values_device."""
+    return hip_lib().tb_hip_int8_values_device(_dev(codes), _dev(scales), _dev(values), rows, k,
+                                               dtype, _stream(stream))
+
+
+def int8_product_device(a_codes, a_scales, a_rows: int, rows, w_codes, w_scales, offsets, bias,
+                        row_scale, out, m: int, n: int, k: int, experts: int, act: int,
+                        dtype: int, stream=None) -> int:
+    """tb_hip_int8_product_device."""
+    return hip_lib().tb_hip_int8_product_device(
+        _dev(a_codes), _dev(a_scales), a_rows, _dev(rows), _dev(w_codes), _dev(w_scales),
+        _dev(offsets), _dev(bias), _dev(row_scale), _dev(out), m, n, k, experts, act, dtype,
+        _stream(stream))
+
+
 __all__ = ["DTYPES", "ACTS", "SCORES", "MX4_BLOCK", "group_norm_workspace_bytes",
            "group_norm_device", "group_norm_backward_device", "route_device",
            "route_backward_device", "expert_order_workspace_bytes", "expert_order_device",
-           "mx4_padded", "mx4_quantise_device", "mx4_values_device", "mx4_product_device"]
+           "mx4_padded", "mx4_quantise_device", "mx4_values_device", "mx4_product_device",
+           "expert_rows_device", "expert_rows_backward_device", "expert_sum_device",
+           "expert_sum_backward_device", "embed_device", "embed_order_workspace_bytes",
+           "embed_order_device", "embed_backward_workspace_bytes", "embed_backward_device",
+           "int8_padded", "int8_quantise_device", "int8_values_device", "int8_product_device"]

@@ -88,6 +88,35 @@ HIP_SIGNATURES = {
     "tb_hip_mx4_product_device":
         (c_int, [c_void_p, c_void_p, c_size_t] + [c_void_p] * 7 +
          [c_size_t, c_size_t, c_size_t, c_int, c_int, c_int, c_void_p]),
+    "tb_hip_expert_rows_device":
+        (c_int, [c_void_p, c_size_t] + [c_void_p] * 4 +
+         [c_size_t, c_int, c_int, c_size_t, c_int, c_void_p]),
+    "tb_hip_expert_rows_backward_device":
+        (c_int, [c_void_p, c_size_t] * 2 + [c_void_p] * 4 +
+         [c_size_t, c_int, c_size_t, c_int, c_void_p]),
+    "tb_hip_expert_sum_device":
+        (c_int, [c_void_p, c_size_t] + [c_void_p] * 3 +
+         [c_size_t, c_void_p, c_size_t, c_int, c_size_t, c_int, c_void_p]),
+    "tb_hip_expert_sum_backward_device":
+        (c_int, [c_void_p, c_size_t] * 2 + [c_void_p] * 5 +
+         [c_size_t, c_int, c_int, c_size_t, c_int, c_void_p]),
+    "tb_hip_embed_device":
+        (c_int, [c_void_p] + [c_void_p, c_size_t] * 2 +
+         [c_float, c_void_p, c_size_t, c_size_t, c_size_t, c_int, c_void_p]),
+    "tb_hip_embed_order_workspace_bytes": (c_size_t, [c_size_t, c_size_t]),
+    "tb_hip_embed_order_device": (c_int, [c_void_p] * 4 + [c_size_t, c_size_t, c_void_p]),
+    "tb_hip_embed_backward_workspace_bytes": (c_size_t, [c_size_t, c_size_t, c_size_t]),
+    "tb_hip_embed_backward_device":
+        (c_int, [c_void_p, c_size_t] + [c_void_p] * 3 + [c_float] + [c_void_p] * 2 +
+         [c_size_t, c_size_t, c_size_t, c_int, c_void_p]),
+    "tb_hip_int8_padded": (c_size_t, [c_size_t]),
+    "tb_hip_int8_quantise_device":
+        (c_int, [c_void_p, c_size_t, c_void_p, c_void_p, c_size_t, c_size_t, c_int, c_void_p]),
+    "tb_hip_int8_values_device":
+        (c_int, [c_void_p] * 3 + [c_size_t, c_size_t, c_int, c_void_p]),
+    "tb_hip_int8_product_device":
+        (c_int, [c_void_p, c_void_p, c_size_t] + [c_void_p] * 7 +
+         [c_size_t, c_size_t, c_size_t, c_int, c_int, c_int, c_void_p]),
 }
 
 SYNTH_SIGNATURES = {
