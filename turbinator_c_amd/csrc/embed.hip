@@ -100,7 +100,7 @@ struct OrderArgs {
     i32x2 *ranges;
     int *counts;            // [segments][digits + 1]
     size_t tokens, entries, segment;
-    unsigned segments;
+    unsigned segments, entry_blocks;
     int shift, bits, last;
 };
 
@@ -117,53 +117,62 @@ __global__ __launch_bounds__(kThreads) void clear_kernel(i32x2 *ranges, size_t e
 }
 
 // Few tokens: a token's place is the number of smaller keys and of equal ones
-// before it.  Each lane has a token, each wave a share of the keys, which come
-// through scalar loads; the shares are added up in LDS.
+// before it, an entry's range what lies below and up to it.  Each lane has a
+// token (or an entry), each wave a share of the keys, which it loads 64 at a
+// time and compares lane by lane; the shares are added up in LDS.
 constexpr int kRankWaves = 16;
 constexpr size_t kRankMost = 4096;
 
-__global__ __launch_bounds__(64 * kRankWaves) void rank_kernel(OrderArgs a) {
+__global__ __launch_bounds__(64 * kRankWaves) void rank_kernel(OrderArgs a, unsigned token_blocks) {
     __shared__ int parts[kRankWaves][3][64];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    const int n = (int)a.tokens, i0 = blockIdx.x * 64, i = i0 + lane;
-    const unsigned key = i < n ? entry_of(a.ids, a.entries, i) : 0;
-    const int per = (n + kRankWaves - 1) / kRankWaves;
-    const int j0 = wave * per, j1 = j0 + per < n ? j0 + per : n;
-    int less = 0, most = 0, place = 0;  // smaller keys, those and equal ones, keys in front
-    const int a0 = j1 < i0 ? j1 : i0;
-    for (int j = j0; j < a0; ++j) {
-        const unsigned o = entry_of(a.ids, a.entries, j);
-        less += o < key;
-        most += o <= key;
+    const bool tokens = blockIdx.x < token_blocks;
+    const int n = (int)a.tokens, last = tokens ? n : (int)a.entries;
+    const int i0 = (tokens ? blockIdx.x : blockIdx.x - token_blocks) * 64, i = i0 + lane;
+    const unsigned key = !tokens ? i : i < n ? entry_of(a.ids, a.entries, i) : 0;
+    // Smaller keys; those and equal ones; keys in front of the token's.
+    int less = 0, most = 0, place = 0;
+    for (int j0 = wave * 64; j0 < n; j0 += 64 * kRankWaves) {
+        const int keys =
+            (int)(j0 + lane < n ? entry_of(a.ids, a.entries, j0 + lane) : 0x7fffffffu);
+        int below = 0, upto = 0, front = 0;
+#pragma unroll 8
+        for (int j = 0; j < 64; ++j) {
+            const unsigned o = (unsigned)__builtin_amdgcn_readlane(keys, j);
+            below += o < key;
+            upto += o <= key;
+        }
+        if (j0 == i0) {
+            // Behind the smaller ones, the lanes in front with the same key.
+            unsigned long long same = ~0ull;
+            for (int bit = 0; bit < a.bits; ++bit) {
+                const bool set = key >> bit & 1;
+                const unsigned long long all = __ballot(set);
+                same &= set ? all : ~all;
+            }
+            front = below + __popcll(same & ((1ull << lane) - 1));
+        }
+        less += below;
+        most += upto;
+        place += j0 == i0 ? front : j0 < i0 ? upto : below;
     }
-    place = most;
-    const int b1 = j1 < i0 + 64 ? j1 : i0 + 64;
-    for (int j = j0 > i0 ? j0 : i0; j < b1; ++j) {
-        const unsigned o = entry_of(a.ids, a.entries, j);
-        less += o < key;
-        most += o <= key;
-        place += o < key || (o == key && j < i);
-    }
-    const int before = less;
-    for (int j = j0 > i0 + 64 ? j0 : i0 + 64; j < j1; ++j) {
-        const unsigned o = entry_of(a.ids, a.entries, j);
-        less += o < key;
-        most += o <= key;
-    }
-    place += less - before;
     parts[wave][0][lane] = less;
     parts[wave][1][lane] = most;
     parts[wave][2][lane] = place;
     __syncthreads();
-    if (wave || i >= n) return;
+    if (wave || i >= last) return;
     for (int w = 1; w < kRankWaves; ++w) {
         less += parts[w][0][lane];
         most += parts[w][1][lane];
         place += parts[w][2][lane];
     }
     const bool known = key < a.entries;
-    a.to[place] = known ? i : -1;
-    if (known && place == less) a.ranges[key] = (i32x2){less, most};
+    if (tokens) a.to[place] = known ? i : -1;
+    // Without workgroups for the entries each one's first token writes its range.
+    if (!tokens)
+        a.ranges[i] = most > less ? (i32x2){less, most} : (i32x2){0, 0};
+    else if (!a.entry_blocks && known && place == less)
+        a.ranges[key] = (i32x2){less, most};
 }
 
 // Many tokens: a stable counting sort by digits, the least first; tokens
@@ -198,19 +207,33 @@ __global__ __launch_bounds__(kSortThreads) void count_kernel(OrderArgs a) {
             a.ranges[v] = (i32x2){0, 0};
 }
 
+// A lane's tokens of one turn and their digits, one past the others behind c1.
+constexpr int kBatch = 4;
+struct Turn {
+    int token[kBatch];
+    unsigned digit[kBatch];
+    __device__ __forceinline__ void load(const OrderArgs &a, size_t c, size_t c1) {
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) {
+            digit[j] = ~0u;
+            if (c + 64 * j < c1) digit[j] = digit_of(a, c + 64 * j, token[j]);
+        }
+    }
+};
+
 __global__ __launch_bounds__(kSortThreads) void place_kernel(OrderArgs a) {
     extern __shared__ int lds[];
     const int digits = (1 << a.bits) + 1, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     int *start = lds, *next = lds + digits * (1 + wave);
     for (int i = threadIdx.x; i < digits * kSortWaves; i += kSortThreads) lds[digits + i] = 0;
-    __syncthreads();
     const size_t run = a.segment / kSortWaves, c0 = blockIdx.x * a.segment + wave * run;
     const size_t c1 = c0 + run < a.tokens ? c0 + run : a.tokens;
-    int token;
-    for (size_t c = c0 + lane; c < c1; c += 64) atomicAdd(&next[digit_of(a, c, token)], 1);
+    Turn now;
+    now.load(a, c0 + lane, c1);
     // Of each digit: all segments' counts, and those of the segments before.
     for (int d = threadIdx.x; d < digits; d += kSortThreads) {
         int all = 0, before = 0;
+#pragma unroll 16
         for (unsigned s = 0; s < a.segments; ++s) {
             const int n = a.counts[(size_t)s * digits + d];
             all += n;
@@ -220,6 +243,12 @@ __global__ __launch_bounds__(kSortThreads) void place_kernel(OrderArgs a) {
         lds[digits * (1 + kSortWaves) + d] = before;
     }
     __syncthreads();
+    for (size_t c = c0; c < c1; c += 64 * kBatch) {
+        if (c > c0) now.load(a, c + lane, c1);
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j)
+            if (now.digit[j] != ~0u) atomicAdd(&next[now.digit[j]], 1);
+    }
     if (wave == 0) {
         int below = 0;
         for (int d0 = 0; d0 < digits; d0 += 64) {
@@ -238,24 +267,28 @@ __global__ __launch_bounds__(kSortThreads) void place_kernel(OrderArgs a) {
         }
     }
     __syncthreads();
-    for (size_t b = c0; b < c1; b += 64) {
-        const bool live = b + lane < c1;
-        unsigned d = 0;
-        if (live) d = digit_of(a, b + lane, token);
-        // The lanes with the same digit.
-        unsigned long long same = __ballot(live);
-        for (int bit = 0; bit <= a.bits; ++bit) {
-            const bool set = d >> bit & 1;
-            const unsigned long long all = __ballot(set);
-            same &= set ? all : ~all;
+    for (size_t c = c0; c < c1; c += 64 * kBatch) {
+        // One turn holds a run of the usual length throughout.
+        if (run > 64 * kBatch) now.load(a, c + lane, c1);
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) {
+            const unsigned d = now.digit[j];
+            const bool live = d != ~0u;
+            // The lanes with the same digit.
+            unsigned long long same = __ballot(live);
+            for (int bit = 0; bit <= a.bits; ++bit) {
+                const bool set = d >> bit & 1;
+                const unsigned long long all = __ballot(set);
+                same &= set ? all : ~all;
+            }
+            const int rank = __popcll(same & ((1ull << lane) - 1));
+            int at = 0;
+            if (live) at = next[d] + rank;
+            wave_fence();
+            if (live && rank == 0) next[d] = at + __popcll(same);
+            wave_fence();
+            if (live) a.to[at] = a.last && d == 1u << a.bits ? -1 : now.token[j];
         }
-        const int rank = __popcll(same & ((1ull << lane) - 1));
-        int at = 0;
-        if (live) at = next[d] + rank;
-        wave_fence();
-        if (live && rank == 0) next[d] = at + __popcll(same);
-        wave_fence();
-        if (live) a.to[at] = a.last && d == 1u << a.bits ? -1 : token;
     }
 }
 
@@ -309,29 +342,37 @@ __device__ __forceinline__ long long entry_at(const GradArgs &a, size_t place) {
     return id >= 0 && (size_t)id < a.entries ? id : -1;
 }
 
-// Adds up element e on of the rows at places b .. end-1 of the order.
+// Adds up element e on of the rows at every `step`th place from b to end of the
+// order, four rows at a time and those in pairs.  More at a time cost registers,
+// and with them waves whose chains of loads (range, places, rows) overlap:
+// 163,840 x 1,024 bf16 to 32,768 entries with their order 162 us, and 166 with
+// two, 183 with eight, 242 with sixteen.
 template <class T, int B>
-__device__ __forceinline__ void add_rows(const GradArgs &a, long long b, long long end, unsigned e,
-                                         float (&sum)[Vec<T, B>::n]) {
+__device__ __forceinline__ void add_rows(const GradArgs &a, long long b, long long end, int step,
+                                         unsigned e, float (&sum)[Vec<T, B>::n]) {
     typedef Vec<T, B> X;
-    constexpr int kAhead = 8;
-    for (; b < end; b += kAhead) {
+    constexpr int kAhead = 4;
+    for (; b < end; b += kAhead * step) {
         typename X::raw row[kAhead];
-        bool there[kAhead];
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) {
-            const int t = a.order[b + i < end ? b + i : end - 1];
-            there[i] = b + i < end && t >= 0 && (size_t)t < a.tokens;
-            if (there[i]) row[i] = load_loose<T, B>(a.dout + (size_t)t * a.stride, e);
+            const long long at = b + i * step;
+            const int t = at < end ? a.order[at] : -1;
+            row[i] = typename X::raw{};
+            if (t >= 0 && (size_t)t < a.tokens)
+                row[i] = load_loose<T, B>(a.dout + (size_t)t * a.stride, e);
         }
+        float x[kAhead][X::n];
 #pragma unroll
-        for (int i = 0; i < kAhead; ++i) {
-            if (!there[i]) continue;
-            float x[X::n];
-            X::unpack(row[i], x);
+        for (int i = 0; i < kAhead; ++i) X::unpack(row[i], x[i]);
 #pragma unroll
-            for (int j = 0; j < X::n; ++j) sum[j] += x[j];
-        }
+        for (int half = kAhead / 2; half; half /= 2)
+#pragma unroll
+            for (int i = 0; i < half; ++i)
+#pragma unroll
+                for (int j = 0; j < X::n; ++j) x[i][j] += x[i + half][j];
+#pragma unroll
+        for (int j = 0; j < X::n; ++j) sum[j] += x[0][j];
     }
 }
 
@@ -369,7 +410,7 @@ __global__ __launch_bounds__(kThreads) void grad_kernel(GradArgs a) {
         if (whole) {
             const i32x2 r = range_of(a, at);
             if (r[1] - r[0] > (int)kChunk) continue;
-            add_rows<T, B>(a, r[0], r[1], e, sum);
+            add_rows<T, B>(a, r[0], r[1], 1, e, sum);
             store_floats<N>(a.dtable + at * a.s.width, e, sum, a.scale);
             continue;
         }
@@ -379,8 +420,8 @@ __global__ __launch_bounds__(kThreads) void grad_kernel(GradArgs a) {
         if (head >= 0) {
             const i32x2 r = range_of(a, head);
             if (r[1] - r[0] > (int)kChunk) {
-                add_rows<T, B>(a, (long long)c0, r[1] < (long long)c1 ? r[1] : (long long)c1, e,
-                               sum);
+                add_rows<T, B>(a, (long long)c0, r[1] < (long long)c1 ? r[1] : (long long)c1, 1,
+                               e, sum);
                 store_floats<N>(part, e, sum, 1.0f);
             }
         }
@@ -388,50 +429,113 @@ __global__ __launch_bounds__(kThreads) void grad_kernel(GradArgs a) {
             const i32x2 r = range_of(a, tail);
             if (r[1] - r[0] > (int)kChunk) {
                 float other[N] = {};
-                add_rows<T, B>(a, r[0] > (long long)c0 ? r[0] : (long long)c0, (long long)c1, e,
-                               other);
+                add_rows<T, B>(a, r[0] > (long long)c0 ? r[0] : (long long)c0, (long long)c1, 1,
+                               e, other);
                 store_floats<N>(part + a.part_width, e, other, 1.0f);
             }
         }
     }
 }
 
-// Joins the parts of the long range that starts in a chunk, if one does: 64
-// columns to a workgroup, 16 lanes of four; 16 parts at a time.
+// Joins the parts of the long ranges: a workgroup has 16 chunks and 64 columns,
+// and finds the ranges that start in its chunks, at most one in each.  Those of
+// a few parts are added up by 16 lanes each, the others by the workgroup.
 constexpr int kJoinLanes = 16, kJoinGroups = kThreads / kJoinLanes, kJoinColumns = 4 * kJoinLanes;
+constexpr int kJoinChunks = 16, kJoinShort = 8;
+static_assert(kJoinChunks <= kJoinGroups);
 
 __global__ __launch_bounds__(kThreads) void join_kernel(GradArgs a) {
     __shared__ f32x4 sums[kJoinGroups][kJoinLanes];
+    __shared__ int entries[kJoinChunks], slots[kJoinChunks], ends[kJoinChunks];
     const size_t slices = (a.s.width + kJoinColumns - 1) / kJoinColumns;
+    const size_t blocks = (a.chunks + kJoinChunks - 1) / kJoinChunks;
     const unsigned lane = threadIdx.x % kJoinLanes, group = threadIdx.x / kJoinLanes;
-    for (size_t item = blockIdx.x; item < a.chunks * slices; item += gridDim.x) {
-        const size_t chunk = item / slices, c0 = chunk * kChunk;
-        const size_t c1 = c0 + kChunk < a.tokens ? c0 + kChunk : a.tokens;
-        const long long entry = entry_at(a, c1 - 1);
-        if (entry < 0) continue;
-        const i32x2 r = range_of(a, entry);
-        if (r[1] - r[0] <= (int)kChunk || (size_t)r[0] < c0 || (size_t)r[0] >= c1) continue;
-        const size_t column = (item - chunk * slices) * kJoinColumns + lane * 4;
-        const size_t last = ((size_t)r[1] - 1) / kChunk;
-        f32x4 sum = {0, 0, 0, 0};
-        if (column < a.part_width)
-#pragma unroll 4
-            for (size_t c = chunk + group; c <= last; c += kJoinGroups) {
-                const size_t slot = c == chunk && (size_t)r[0] > c0;
-                sum += *reinterpret_cast<const f32x4 *>(a.parts + (2 * c + slot) * a.part_width +
-                                                        column);
+    for (size_t item = blockIdx.x; item < blocks * slices; item += gridDim.x) {
+        const size_t first = item / slices * kJoinChunks;
+        const size_t column = item % slices * kJoinColumns + lane * 4;
+        if (threadIdx.x < kJoinChunks) {
+            const size_t chunk = first + threadIdx.x, c0 = chunk * kChunk;
+            entries[threadIdx.x] = -1;
+            if (chunk < a.chunks) {
+                const size_t c1 = c0 + kChunk < a.tokens ? c0 + kChunk : a.tokens;
+                const long long entry = entry_at(a, c1 - 1);
+                const i32x2 r = entry < 0 ? (i32x2){0, 0} : range_of(a, entry);
+                if (r[1] - r[0] > (int)kChunk && (size_t)r[0] >= c0 && (size_t)r[0] < c1) {
+                    entries[threadIdx.x] = (int)entry;
+                    // The first chunk's sum is its second one unless the range fills it.
+                    slots[threadIdx.x] = (size_t)r[0] > c0;
+                    ends[threadIdx.x] = (int)(((size_t)r[1] - 1) / kChunk - chunk) + 1;
+                }
             }
-        sums[group][lane] = sum;
+        }
         __syncthreads();
-        if (threadIdx.x < kJoinColumns) {
-            const size_t c = (item - chunk * slices) * kJoinColumns + threadIdx.x;
-            float all = 0.0f;
-            for (int g = 0; g < kJoinGroups; ++g)
-                all += sums[g][threadIdx.x / 4][threadIdx.x % 4];
-            if (c < a.s.width) a.dtable[(size_t)entry * a.s.width + c] = all * a.scale;
+        // Sums parts b, b + step, .. of a range that starts in chunk first + i.
+        auto add = [&](int i, int b, int step) {
+            f32x4 sum = {0, 0, 0, 0};
+            if (column < a.part_width)
+#pragma unroll 4
+                for (int c = b; c < ends[i]; c += step) {
+                    const size_t slot = 2 * (first + i + c) + (c ? 0 : slots[i]);
+                    sum += *reinterpret_cast<const f32x4 *>(a.parts + slot * a.part_width + column);
+                }
+            return sum;
+        };
+        auto write = [&](int i, f32x4 sum) {
+            float *row = a.dtable + (size_t)entries[i] * a.s.width + column;
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (column + j < a.s.width) row[j] = sum[j] * a.scale;
+        };
+        if (group < kJoinChunks && entries[group] >= 0 && ends[group] <= kJoinShort)
+            write(group, add(group, 0, 1));
+        for (int i = 0; i < kJoinChunks; ++i) {
+            if (entries[i] < 0 || ends[i] <= kJoinShort) continue;
+            sums[group][lane] = add(i, group, kJoinGroups);
+            __syncthreads();
+            if (group == 0) {
+                f32x4 sum = sums[0][lane];
+                for (int g = 1; g < kJoinGroups; ++g) sum += sums[g][lane];
+                write(i, sum);
+            }
+            __syncthreads();
         }
         __syncthreads();
     }
+}
+
+// Few tokens and entries: a workgroup has an entry's row or a piece of it, its
+// groups of lanes every so manieth token; their sums meet in LDS, in pairs.
+// One launch instead of two.
+constexpr int kSmallThreads = 1024;
+constexpr size_t kSmallTokens = 4096, kSmallItems = 4096;
+
+template <class T, int B>
+__global__ __launch_bounds__(kSmallThreads) void small_kernel(GradArgs a) {
+    constexpr int N = Vec<T, B>::n;
+    __shared__ float sums[N][kSmallThreads];
+    const unsigned lane = threadIdx.x & (a.s.lanes - 1), group = threadIdx.x / a.s.lanes;
+    const unsigned groups = kSmallThreads / a.s.lanes;
+    const size_t entry = blockIdx.x / a.s.pieces;
+    const unsigned v = (unsigned)(blockIdx.x - entry * a.s.pieces) * a.s.lanes + lane;
+    const bool there = v < a.s.vectors;
+    const unsigned e = there ? first_of<N>(a.s, v) : 0;
+    const i32x2 r = range_of(a, entry);
+    float sum[N] = {};
+    if (there) add_rows<T, B>(a, r[0] + (int)group, r[1], groups, e, sum);
+    const unsigned used = r[1] - r[0] < (int)groups ? r[1] > r[0] ? r[1] - r[0] : 0 : groups;
+    unsigned half = 1;
+    while (half < used) half *= 2;
+    for (half /= 2; half; half /= 2) {
+        __syncthreads();
+        if (group >= half && group < 2 * half)
+#pragma unroll
+            for (int i = 0; i < N; ++i) sums[i][threadIdx.x] = sum[i];
+        __syncthreads();
+        if (group < half)
+#pragma unroll
+            for (int i = 0; i < N; ++i) sum[i] += sums[i][threadIdx.x + half * a.s.lanes];
+    }
+    if (group == 0 && there) store_floats<N>(a.dtable + entry * a.s.width, e, sum, a.scale);
 }
 
 // --------------------------------------------------------------------------
@@ -500,6 +604,11 @@ template <class T, int B>
 void launch_grad(GradArgs &a, hipStream_t q) {
     a.s = shape_of<T, B>(a.s.width);
     const size_t per = kThreads / a.s.lanes;
+    if (a.tokens <= kSmallTokens && a.entries * a.s.pieces <= kSmallItems) {
+        const unsigned items = (unsigned)(a.entries * a.s.pieces);
+        small_kernel<T, B><<<items, kSmallThreads, 0, q>>>(a);
+        return;
+    }
     // Chunks that no range is longer than need no joining.
     const bool join = a.tokens > kChunk;
     a.chunk_blocks = join ? grid_of(a.chunks * a.s.pieces, per) : 0;
@@ -512,7 +621,8 @@ void launch_grad(GradArgs &a, hipStream_t q) {
     if (!wide) grad_kernel<T, B, 0><<<grid, kThreads, 0, q>>>(a);
     if (join) {
         const size_t slices = (a.s.width + kJoinColumns - 1) / kJoinColumns;
-        join_kernel<<<grid_of(a.chunks * slices, 1), kThreads, 0, q>>>(a);
+        const size_t blocks = (a.chunks + kJoinChunks - 1) / kJoinChunks;
+        join_kernel<<<grid_of(blocks * slices, 1), kThreads, 0, q>>>(a);
     }
 }
 
@@ -578,8 +688,13 @@ extern "C" int tb_hip_embed_order_device(const int *ids, int *order, int *ranges
     hipStream_t q = reinterpret_cast<hipStream_t>(stream);
     (void)hipGetLastError();
     if (tokens <= kRankMost) {
-        clear_kernel<<<grid_of(entries, kThreads), kThreads, 0, q>>>(a.ranges, entries);
-        rank_kernel<<<(unsigned)((tokens + 63) / 64), 64 * kRankWaves, 0, q>>>(a);
+        const unsigned blocks = (unsigned)((tokens + 63) / 64);
+        a.bits = log2_up(entries + 1);
+        if (entries <= kRankMost)
+            a.entry_blocks = (unsigned)((entries + 63) / 64);
+        else
+            clear_kernel<<<grid_of(entries, kThreads), kThreads, 0, q>>>(a.ranges, entries);
+        rank_kernel<<<blocks + a.entry_blocks, 64 * kRankWaves, 0, q>>>(a, blocks);
         return hipGetLastError() == hipSuccess;
     }
     const SortShape s = sort_shape(tokens, entries);
