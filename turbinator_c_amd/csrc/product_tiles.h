@@ -1,6 +1,6 @@
 // What the products of quantised rows share: which rows a tile of the output
-// has, loads that write LDS themselves, and stores of whole runs.  `Args` has
-// the products' offsets, m, n, experts, out and vector.
+// has, and how many of them pass through LDS at a time.  `Args` has the
+// products' offsets, m and experts.
 #pragma once
 
 #include "layer_math.h"
@@ -56,43 +56,11 @@ __device__ __forceinline__ bool find_rows(const Args &a, size_t tile, int height
     return false;
 }
 
-typedef const __attribute__((address_space(1))) void *GlobalPtr;
 typedef __attribute__((address_space(3))) void *LdsPtr;
-
-__device__ __forceinline__ void load_to_lds(const void *from, void *to) {
-    __builtin_amdgcn_global_load_lds((GlobalPtr)from, (LdsPtr)to, 16, 0, 0);
-}
-
-// Waits for the wave's loads and LDS accesses, then for the other waves.
-__device__ __forceinline__ void arrive() {
-    asm volatile("" ::: "memory");
-    __builtin_amdgcn_sched_barrier(0);
-    __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0)
-    __builtin_amdgcn_s_barrier();
-    __builtin_amdgcn_sched_barrier(0);
-    asm volatile("" ::: "memory");
-}
 
 // The most row tiles, halving from `all`, whose `bytes` each fit into `room`.
 constexpr int pass_tiles(int all, int bytes, int room) {
     return all * bytes <= room ? all : pass_tiles(all / 2, bytes, room);
-}
-
-// 16 bytes of columns from n0 on of row r.  Nothing here reads them again:
-// stores past the caches (8,192 x 2,048 results, k 1,024: 20.7 us, else 22.4).
-template <class T, class Args>
-__device__ __forceinline__ void store_run(const Args &a, size_t r, size_t n0, u32x4 run) {
-    constexpr int kRun = 16 / sizeof(T);
-    T *out = reinterpret_cast<T *>(a.out) + r * a.n + n0;
-    if (a.vector) {  // rows hold whole runs
-        __builtin_nontemporal_store(run, reinterpret_cast<u32x4 *>(out));
-    } else {
-        typedef T elems __attribute__((ext_vector_type(kRun)));
-        const elems v = __builtin_bit_cast(elems, run);
-#pragma unroll
-        for (int i = 0; i < kRun; ++i)
-            if (n0 + i < a.n) out[i] = v[i];
-    }
 }
 
 }  // namespace layer
