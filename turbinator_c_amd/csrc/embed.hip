@@ -57,6 +57,7 @@ struct LookupArgs {
     char *out;
     size_t table_stride, base_stride, tokens, entries;
     float scale;
+    bool stream;  // base past the caches
     RowShape s;
 };
 
@@ -77,7 +78,10 @@ __global__ __launch_bounds__(kThreads) void lookup_kernel(LookupArgs a) {
         const unsigned e = first_of<X::n>(a.s, v);
         const int id = a.ids[t];
         raw out = {};
-        if (a.base) out = load_loose<T, B>(a.base + t * a.base_stride, e);
+        if (a.base && a.stream)
+            out = stream_in<T, B>(a.base + t * a.base_stride, e);
+        else if (a.base)
+            out = load_loose<T, B>(a.base + t * a.base_stride, e);
         if (id >= 0 && (size_t)id < a.entries) {
             float x[X::n], y[X::n];
             X::unpack(load_loose<T, B>(a.table + (size_t)id * a.table_stride, e), x);
@@ -87,7 +91,7 @@ __global__ __launch_bounds__(kThreads) void lookup_kernel(LookupArgs a) {
                 y[i] = a.base ? fmaf(a.scale, x[i], y[i]) : a.scale * x[i];
             out = X::pack(y);
         }
-        store_loose<T, B>(a.out + t * row_bytes, e, out);
+        stream_out<T, B>(a.out + t * row_bytes, e, out);
     }
 }
 
@@ -347,7 +351,7 @@ __device__ __forceinline__ long long entry_at(const GradArgs &a, size_t place) {
 // and with them waves whose chains of loads (range, places, rows) overlap:
 // 163,840 x 1,024 bf16 to 32,768 entries with their order 162 us, and 166 with
 // two, 183 with eight, 242 with sixteen.
-template <class T, int B>
+template <class T, int B, bool STREAM>
 __device__ __forceinline__ void add_rows(const GradArgs &a, long long b, long long end, int step,
                                          unsigned e, float (&sum)[Vec<T, B>::n]) {
     typedef Vec<T, B> X;
@@ -358,9 +362,10 @@ __device__ __forceinline__ void add_rows(const GradArgs &a, long long b, long lo
         for (int i = 0; i < kAhead; ++i) {
             const long long at = b + i * step;
             const int t = at < end ? a.order[at] : -1;
+            const char *from = a.dout + (size_t)t * a.stride;
             row[i] = typename X::raw{};
             if (t >= 0 && (size_t)t < a.tokens)
-                row[i] = load_loose<T, B>(a.dout + (size_t)t * a.stride, e);
+                row[i] = STREAM ? stream_in<T, B>(from, e) : load_loose<T, B>(from, e);
         }
         float x[kAhead][X::n];
 #pragma unroll
@@ -390,7 +395,8 @@ __device__ __forceinline__ void store_floats(float *row, unsigned e, const float
     }
 }
 
-template <class T, int B, int LANES>
+// STREAM: dout is read past the caches.
+template <class T, int B, int LANES, bool STREAM>
 __global__ __launch_bounds__(kThreads) void grad_kernel(GradArgs a) {
     constexpr int N = Vec<T, B>::n;
     const unsigned lanes = LANES ? LANES : a.s.lanes, lane = threadIdx.x & (lanes - 1);
@@ -410,7 +416,7 @@ __global__ __launch_bounds__(kThreads) void grad_kernel(GradArgs a) {
         if (whole) {
             const i32x2 r = range_of(a, at);
             if (r[1] - r[0] > (int)kChunk) continue;
-            add_rows<T, B>(a, r[0], r[1], 1, e, sum);
+            add_rows<T, B, STREAM>(a, r[0], r[1], 1, e, sum);
             store_floats<N>(a.dtable + at * a.s.width, e, sum, a.scale);
             continue;
         }
@@ -420,7 +426,7 @@ __global__ __launch_bounds__(kThreads) void grad_kernel(GradArgs a) {
         if (head >= 0) {
             const i32x2 r = range_of(a, head);
             if (r[1] - r[0] > (int)kChunk) {
-                add_rows<T, B>(a, (long long)c0, r[1] < (long long)c1 ? r[1] : (long long)c1, 1,
+                add_rows<T, B, STREAM>(a, (long long)c0, r[1] < (long long)c1 ? r[1] : (long long)c1, 1,
                                e, sum);
                 store_floats<N>(part, e, sum, 1.0f);
             }
@@ -429,7 +435,7 @@ __global__ __launch_bounds__(kThreads) void grad_kernel(GradArgs a) {
             const i32x2 r = range_of(a, tail);
             if (r[1] - r[0] > (int)kChunk) {
                 float other[N] = {};
-                add_rows<T, B>(a, r[0] > (long long)c0 ? r[0] : (long long)c0, (long long)c1, 1,
+                add_rows<T, B, STREAM>(a, r[0] > (long long)c0 ? r[0] : (long long)c0, (long long)c1, 1,
                                e, other);
                 store_floats<N>(part + a.part_width, e, other, 1.0f);
             }
@@ -521,7 +527,7 @@ __global__ __launch_bounds__(kSmallThreads) void small_kernel(GradArgs a) {
     const unsigned e = there ? first_of<N>(a.s, v) : 0;
     const i32x2 r = range_of(a, entry);
     float sum[N] = {};
-    if (there) add_rows<T, B>(a, r[0] + (int)group, r[1], groups, e, sum);
+    if (there) add_rows<T, B, false>(a, r[0] + (int)group, r[1], groups, e, sum);
     const unsigned used = r[1] - r[0] < (int)groups ? r[1] > r[0] ? r[1] - r[0] : 0 : groups;
     unsigned half = 1;
     while (half < used) half *= 2;
@@ -591,6 +597,7 @@ size_t part_width(size_t width) { return (width + 3) / 4 * 4; }
 template <class T, int B>
 void launch_lookup(LookupArgs &a, hipStream_t q) {
     a.s = shape_of<T, B>(a.s.width);
+    a.stream = a.tokens * a.s.width * sizeof(T) > kStreamBytes;
     const unsigned grid = grid_of(a.tokens * a.s.pieces, kThreads / a.s.lanes);
     if constexpr (B == 16)
         if (a.s.lanes == 64) {
@@ -603,6 +610,7 @@ void launch_lookup(LookupArgs &a, hipStream_t q) {
 template <class T, int B>
 void launch_grad(GradArgs &a, hipStream_t q) {
     a.s = shape_of<T, B>(a.s.width);
+    const bool stream = B == 16 && a.tokens * a.s.width * sizeof(T) > kStreamBytes;
     const size_t per = kThreads / a.s.lanes;
     if (a.tokens <= kSmallTokens && a.entries * a.s.pieces <= kSmallItems) {
         const unsigned items = (unsigned)(a.entries * a.s.pieces);
@@ -613,12 +621,14 @@ void launch_grad(GradArgs &a, hipStream_t q) {
     const bool join = a.tokens > kChunk;
     a.chunk_blocks = join ? grid_of(a.chunks * a.s.pieces, per) : 0;
     const unsigned grid = grid_of(a.entries * a.s.pieces, per) + (unsigned)a.chunk_blocks;
-    bool wide = false;
-    if constexpr (B == 16) {
-        wide = a.s.lanes == 64;
-        if (wide) grad_kernel<T, B, 64><<<grid, kThreads, 0, q>>>(a);
-    }
-    if (!wide) grad_kernel<T, B, 0><<<grid, kThreads, 0, q>>>(a);
+    constexpr int kWide = B == 16 ? 64 : 0;
+    constexpr bool kStreams = B == 16;
+    auto launch = [&](auto kernel) { kernel<<<grid, kThreads, 0, q>>>(a); };
+    if (a.s.lanes == 64)
+        stream ? launch(grad_kernel<T, B, kWide, kStreams>)
+               : launch(grad_kernel<T, B, kWide, false>);
+    else
+        stream ? launch(grad_kernel<T, B, 0, kStreams>) : launch(grad_kernel<T, B, 0, false>);
     if (join) {
         const size_t slices = (a.s.width + kJoinColumns - 1) / kJoinColumns;
         const size_t blocks = (a.chunks + kJoinChunks - 1) / kJoinChunks;

@@ -46,14 +46,14 @@ struct Eight {
     u32x4 part[kParts];
 
     // Values 8 p .. 8 p + 7 of a row, 0 past its end.
+    template <bool STREAM>
     __device__ __forceinline__ void load(const QuantArgs &a, const char *row, unsigned p) {
         const unsigned k0 = p * 8;
         if (k0 + 8 <= a.k) {
 #pragma unroll
-            for (int i = 0; i < kParts; ++i) {
-                const size_t at = (size_t)(k0 + i * X::n) * sizeof(T);
-                part[i] = __builtin_nontemporal_load(reinterpret_cast<const Loose<T, 16> *>(row + at));
-            }
+            for (int i = 0; i < kParts; ++i)
+                part[i] = STREAM ? stream_in<T, 16>(row, k0 + i * X::n)
+                                 : load_loose<T, 16>(row, k0 + i * X::n);
             return;
         }
 #pragma unroll
@@ -131,8 +131,9 @@ __device__ __forceinline__ unsigned wave_most(unsigned v) {
 
 constexpr int kHeld = 4;  // pieces that a lane keeps
 
-// THREADS: a row's, 64 or the workgroup's.
-template <class T, int THREADS>
+// THREADS: a row's, 64 or the workgroup's.  STREAM: the first loads go past the
+// caches.
+template <class T, int THREADS, bool STREAM>
 __global__ __launch_bounds__(kQuantThreads) void quantise_kernel(QuantArgs a) {
     __shared__ unsigned mosts[kQuantThreads / 64];
     constexpr int kRows = kQuantThreads / THREADS;
@@ -144,12 +145,12 @@ __global__ __launch_bounds__(kQuantThreads) void quantise_kernel(QuantArgs a) {
         unsigned most = 0;
 #pragma unroll
         for (int h = 0; h < kHeld; ++h)
-            if (t + h * THREADS < a.pieces) held[h].load(a, row, t + h * THREADS);
+            if (t + h * THREADS < a.pieces) held[h].template load<STREAM>(a, row, t + h * THREADS);
 #pragma unroll
         for (int h = 0; h < kHeld; ++h)
             if (t + h * THREADS < a.pieces) most = held[h].most(most);
         for (unsigned p = t + kHeld * THREADS; p < a.pieces; p += THREADS) {
-            other.load(a, row, p);
+            other.template load<false>(a, row, p);
             most = other.most(most);
         }
         most = wave_most<T>(most);
@@ -171,7 +172,7 @@ __global__ __launch_bounds__(kQuantThreads) void quantise_kernel(QuantArgs a) {
         for (int h = 0; h < kHeld; ++h)
             if (t + h * THREADS < a.pieces) write(t + h * THREADS, held[h]);
         for (unsigned p = t + kHeld * THREADS; p < a.pieces; p += THREADS) {
-            other.load(a, row, p);
+            other.template load<false>(a, row, p);
             write(p, other);
         }
         if (t == 0) a.scales[r] = scale;
@@ -338,7 +339,7 @@ __device__ __forceinline__ void store_columns(const ProductArgs &a, size_t r, si
     constexpr int kRun = 16 / sizeof(T);
     T *out = reinterpret_cast<T *>(a.out) + r * a.n + n0;
     if (n0 + kRun <= a.n) {
-        __builtin_nontemporal_store(run, reinterpret_cast<Loose<T, 16> *>(out));
+        stream_out<T, 16>(reinterpret_cast<char *>(out), 0, run);
     } else {
         typedef T elems __attribute__((ext_vector_type(kRun)));
         const elems v = __builtin_bit_cast(elems, run);
@@ -702,12 +703,24 @@ unsigned grid_of(size_t items, size_t per) {
     return (unsigned)(want < kMaxGrid ? want : kMaxGrid);
 }
 
+template <class T, bool STREAM>
+void launch_rows(const QuantArgs &a, hipStream_t q) {
+    const size_t per = a.pieces <= 64 * kHeld ? kQuantThreads / 64 : 1;
+    const unsigned grid = grid_of(a.rows, per);
+    if (per > 1)
+        quantise_kernel<T, 64, STREAM><<<grid, kQuantThreads, 0, q>>>(a);
+    else
+        quantise_kernel<T, kQuantThreads, STREAM><<<grid, kQuantThreads, 0, q>>>(a);
+}
+
 template <class T>
 void launch_quantise(const QuantArgs &a, hipStream_t q) {
-    if (a.pieces <= 64 * kHeld)
-        quantise_kernel<T, 64><<<grid_of(a.rows, kQuantThreads / 64), kQuantThreads, 0, q>>>(a);
+    // Of longer rows than a workgroup holds the rest is read twice.
+    const bool held = a.pieces <= kQuantThreads * kHeld;
+    if (held && a.rows * a.k * sizeof(T) > kStreamBytes)
+        launch_rows<T, true>(a, q);
     else
-        quantise_kernel<T, kQuantThreads><<<grid_of(a.rows, 1), kQuantThreads, 0, q>>>(a);
+        launch_rows<T, false>(a, q);
 }
 
 bool rows_ok(size_t rows, size_t k, int dtype) {
