@@ -128,11 +128,7 @@ __global__ __launch_bounds__(kThreads) void token_kernel(TokenArgs a) {
                             for (int i = 0; i < X::n; ++i) y[i] = w[j] * x[i];
                             out = X::pack(y);
                         }
-                        char *to = a.rows_out + at[j] * row_bytes;
-                        if (KIND == kRows)
-                            stream_out<T, B>(to, e, out);
-                        else
-                            store_loose<T, B>(to, e, out);
+                        stream_out<T, B>(a.rows_out + at[j] * row_bytes, e, out);
                     }
                 }
                 if (KIND == kRowsBack)
