@@ -286,7 +286,8 @@ int tb_hip_int8_quantise_device(const void *x, size_t row_stride, void *codes, f
                                 size_t rows, size_t k, int dtype, void *stream);
 
 /* The values [rows, k] (dense) that codes and scales stand for, rounded to
- * fp32 and to the type (f16 can overflow).
+ * fp32 and to the type, in which they can overflow (f16; the others within half
+ * a step of their largest).
  * Both return 0 for NULL pointers, rows 0 or above 0x7fffffff, k 0 or above
  * TB_HIP_INT8_MAX_K, an unknown dtype or misaligned pointers or stride. */
 int tb_hip_int8_values_device(const void *codes, const float *scales, void *values, size_t rows,
