@@ -227,6 +227,7 @@ struct ProductArgs {
     char *out;
     size_t a_rows, m, n, kp;
     int experts;
+    bool direct;  // results leave from registers
 };
 
 __device__ __forceinline__ i32x4 step_of(i32x4 w, i32x4 x, i32x4 c) {
@@ -330,7 +331,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_kernel(ProductArgs a) {
 // 12 (8 out of the last cache), start, activation and stores 10: an operation on
 // every output costs 0.5 us, GELU 8.  Tried and not faster: slices of one step in
 // four buffers, three buffers under tiles of 128 rows, rows touched ahead to have
-// them in the L2, results stored from registers in pieces of 16 bytes.
+// them in the L2.
 // 16 bytes of columns from n0 on of row r, past the caches: nothing here reads
 // them again (16,384 x 4,096 x 4,096: 232 us, with ordinary stores 250).
 template <class T>
@@ -382,6 +383,25 @@ __device__ __forceinline__ void multiply(const Operands<MT, NT> &o, i32x4 (&acc)
     for (int i = 0; i < NT; ++i)
 #pragma unroll
         for (int j = 0; j < MT; ++j) acc[i][j] = step_of(o.w[i], o.x[j], acc[i][j]);
+}
+
+// The column of a wave's that row `low` of column tile i's operand is.  Of 16-bit
+// results a lane ends with 16 bytes of consecutive columns in two tiles, the four
+// lanes of a row with 64 bytes; where rows start on 64 bytes they leave from
+// registers (8,192 tokens to 2 of 8 experts, 2,048 x 1,024, with quantisation: 61
+// us, through LDS 64), else through LDS (12,000 x 1,500 x 700: 30 us, from
+// registers 37), as 32-bit results do (8,000 x 2,048 x 1,000: 35 us, from
+// registers 40).  spread_of: where the swizzle puts a column's codes, for such
+// reads.
+template <class T>
+__device__ __forceinline__ int column_of(int i, int low) {
+    if (sizeof(T) == 4) return 16 * i + low;
+    return 32 * (i / 2) + 8 * (low / 4) + 4 * (i % 2) + low % 4;
+}
+template <class T>
+__device__ __forceinline__ int spread_of(int row) {
+    if (sizeof(T) == 4) return row & 7;
+    return (row & 3) | (row >> 3 & 1) << 2;
 }
 
 template <class T, int ACT, int WM, int WN, int MT, int NT, int STAGES>
@@ -455,7 +475,9 @@ __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(ProductArgs a) {
     unsigned from[kLoads];
 #pragma unroll
     for (int i = 0; i < kLoads; ++i)
-        from[i] = row_code[row0 + i * 8 + (lane >> 3)] + ((lane & 7) ^ (lane >> 3));
+        from[i] = row_code[row0 + i * 8 + (lane >> 3)] +
+                  ((lane & 7) ^ (row0 + i * 8 >= BM ? spread_of<T>(row0 + i * 8 - BM + (lane >> 3))
+                                                    : lane >> 3));
     const unsigned slices = (unsigned)(a.kp / kPad);
     const unsigned char *a_base = a.a_codes + a_first * a.kp, *w_base = a.w_codes + w_first * a.kp;
     const unsigned lds = (unsigned)(uintptr_t)(LdsPtr)codes;
@@ -466,13 +488,20 @@ __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(ProductArgs a) {
     };
     const int row_x = wm * MT * 16, row_w = BM + wn * NT * 16;
     const int lane_row = low * kPad, slot = (part ^ (low & 7)) * 16;
+    const int w_row = column_of<T>(0, low), w_slot = (part ^ spread_of<T>(w_row)) * 16;
+    const int w_slot1 = (part ^ spread_of<T>(column_of<T>(1, low))) * 16;
     // Read `r` of a step's operands, the rows' first.
     auto read_one = [&](unsigned stage, int s, Operands<MT, NT> &o, int r) {
-        const unsigned char *p = codes + stage + lane_row + (slot ^ (s * kStep));
-        if (r < MT)
+        if (r < MT) {
+            const unsigned char *p = codes + stage + lane_row + (slot ^ (s * kStep));
             o.x[r] = *reinterpret_cast<const i32x4 *>(p + (row_x + r * 16) * kPad);
-        else
-            o.w[r - MT] = *reinterpret_cast<const i32x4 *>(p + (row_w + (r - MT) * 16) * kPad);
+        } else {
+            const int i = r - MT;
+            const unsigned char *p = codes + stage + w_row * kPad +
+                                     ((i % 2 ? w_slot1 : w_slot) ^ (s * kStep));
+            o.w[i] = *reinterpret_cast<const i32x4 *>(
+                p + (row_w + column_of<T>(i, 0)) * kPad);
+        }
     };
     Operands<MT, NT> even, odd;
 #pragma unroll
@@ -539,52 +568,77 @@ __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(ProductArgs a) {
     for (; slice + STAGES < slices; ++slice) turn(Int<1>(), slice);
     for (; slice + 1 < slices; ++slice) turn(Int<0>(), slice);
     multiply<MT, NT>(odd, acc);
-    arrive_but<0>();
 
-    // Results through LDS, whose rows leave in runs: kPass rows of the tile at a
-    // time, the arrays in turn, so that a pass is read before the next but one
-    // is written.  A lane's four columns are one piece; piece c of a wave's row
-    // r lies at c ^ 4 r, so that the rows of a write fall on different banks.
-    typedef Vec<T, 4 * sizeof(T)> Four;
-    constexpr int kPassTiles = pass_tiles(MT, WM * 16 * BN * sizeof(T), (int)kStage);
-    constexpr int kPass = kPassTiles * WM * 16, kPieces = BN / 4;
-    constexpr int kRun = 16 / sizeof(T), kAcross = BN / kRun, kSweep = kThreads / kAcross;
-    static_assert(MT % kPassTiles == 0);
-    const int c = t % kAcross * kRun;
-    const size_t n1 = n0 + c;
+    // Columns of row `in` of the tile that the lane holds in row tile j.
     const bool weighted = a.rows || a.row_scale;
     f32x4 bias[NT], column[NT];
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
-        bias[i] = *reinterpret_cast<const f32x4 *>(bias_of + (wn * NT + i) * 16 + part * 4);
-        column[i] = *reinterpret_cast<const f32x4 *>(scale_of + (wn * NT + i) * 16 + part * 4);
+        const int c = wn * NT * 16 + column_of<T>(i, part * 4);
+        bias[i] = *reinterpret_cast<const f32x4 *>(bias_of + c);
+        column[i] = *reinterpret_cast<const f32x4 *>(scale_of + c);
     }
+    auto results = [&](int j, int in, float (&v)[NT][4]) {
+        const float row_scale = scale_of_row[in];
 #pragma unroll
-    for (int j0 = 0; j0 < MT; j0 += kPassTiles) {
-        unsigned char *results = codes + j0 / kPassTiles % 2 * kStage;
+        for (int i = 0; i < NT; ++i)
 #pragma unroll
-        for (int j = 0; j < kPassTiles; ++j) {
-            const int in = (wm * MT + j0 + j) * 16 + low, at = (wm * kPassTiles + j) * 16 + low;
-            const float row_scale = scale_of_row[in];
-            float v[NT][4];
+            for (int q = 0; q < 4; ++q)
+                v[i][q] = act_of<kFine<T>, ACT>(
+                    fmaf((float)acc[i][j][q] * row_scale, column[i][q], bias[i][q]));
+        if (weighted) {
+            const float weight = weight_of_row[in];
+            const bool there = real_row[in];
 #pragma unroll
             for (int i = 0; i < NT; ++i)
 #pragma unroll
-                for (int q = 0; q < 4; ++q)
-                    v[i][q] = act_of<kFine<T>, ACT>(
-                        fmaf((float)acc[i][j0 + j][q] * row_scale, column[i][q], bias[i][q]));
-            if (weighted) {
-                const float weight = weight_of_row[in];
-                const bool there = real_row[in];
+                for (int q = 0; q < 4; ++q) v[i][q] = there ? v[i][q] * weight : 0.0f;
+        }
+    };
+    constexpr int kRun = 16 / sizeof(T);
+    if (sizeof(T) == 2 && a.direct) {
 #pragma unroll
-                for (int i = 0; i < NT; ++i)
+        for (int j = 0; j < MT; ++j) {
+            const int in = (wm * MT + j) * 16 + low;
+            float v[NT][4];
+            results(j, in, v);
+            if (in >= height) continue;
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) v[i][q] = there ? v[i][q] * weight : 0.0f;
+            for (int i = 0; i < NT; i += 2) {
+                float run[kRun];
+#pragma unroll
+                for (int q = 0; q < kRun; ++q) run[q] = v[i + q / 4][q % 4];
+                const size_t c = n0 + wn * NT * 16 + column_of<T>(i, part * 4);
+                if (c < a.n) store_columns<T>(a, m0 + in, c, Vec<T, 16>::pack(run));
             }
+        }
+        return;
+    }
+    arrive_but<0>();
+    // Through LDS, whose rows leave in runs: kPass rows of the tile at a time, two
+    // buffers in turn, so that a pass is read before the next but one is written.
+    // Four columns are one piece; piece c of a wave's row r lies at c ^ 4 r, so
+    // that the rows of a write fall on different banks.
+    typedef Vec<T, 4 * sizeof(T)> Four;
+    constexpr int kPassTiles = pass_tiles(MT, WM * 16 * BN * sizeof(T), (int)kStage);
+    constexpr int kPass = kPassTiles * WM * 16, kPieces = BN / 4;
+    constexpr int kAcross = BN / kRun, kSweep = kThreads / kAcross;
+    static_assert(MT % kPassTiles == 0);
+    const int c = t % kAcross * kRun;
+    const size_t n1 = n0 + c;
+#pragma unroll
+    for (int j0 = 0; j0 < MT; j0 += kPassTiles) {
+        unsigned char *passed = codes + j0 / kPassTiles % 2 * kStage;
+#pragma unroll
+        for (int j = 0; j < kPassTiles; ++j) {
+            const int at = (wm * kPassTiles + j) * 16 + low;
+            float v[NT][4];
+            results(j0 + j, (wm * MT + j0 + j) * 16 + low, v);
 #pragma unroll
             for (int i = 0; i < NT; ++i) {
-                const int piece = ((wn * NT + i) * 4 + part) ^ (low * 4 & (kPieces - 1));
-                reinterpret_cast<typename Four::raw *>(results)[at * kPieces + piece] =
+                const int piece = ((wn * NT * 16 + column_of<T>(i, part * 4)) / 4) ^
+                                  (low * 4 & (kPieces - 1));
+                reinterpret_cast<typename Four::raw *>(passed)[at * kPieces + piece] =
                     Four::pack(v[i]);
             }
         }
@@ -595,7 +649,7 @@ __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(ProductArgs a) {
             const int in = row / (kPassTiles * 16) * (MT * 16) + j0 * 16 + row % (kPassTiles * 16);
             const int piece = c / 4 ^ (row % 16 * 4 & (kPieces - 1));
             const u32x4 run = *reinterpret_cast<const u32x4 *>(
-                results + (row * kPieces + piece) * sizeof(typename Four::raw));
+                passed + (row * kPieces + piece) * sizeof(typename Four::raw));
             if (in < height) store_columns<T>(a, m0 + in, n1, run);
         }
     }
@@ -812,6 +866,7 @@ extern "C" int tb_hip_int8_product_device(const void *a_codes, const float *a_sc
     a.n = n;
     a.kp = padded(k);
     a.experts = experts;
+    a.direct = dtype != TB_HIP_F32 && multiple_of(out, 64) && n * type_size(dtype) % 64 == 0;
     hipStream_t q = reinterpret_cast<hipStream_t>(stream);
     (void)hipGetLastError();
     const int shape = shape_for(a);
