@@ -162,6 +162,14 @@ def test_long_orders(torch_cuda, t, entries):
         check_order(ids_of(g, t, entries, kind), entries)
 
 
+@pytest.mark.parametrize("kind", ["even", "skewed", "one", "none", "rising", "outside"])
+@pytest.mark.parametrize("entries", [1, 127, 128, 4096, 4097, 2 ** 20])
+@pytest.mark.parametrize("t", [63, 65, 2047, 2049, 3000, 4095])
+def test_short_orders(torch_cuda, t, entries, kind):
+    """Around the bounds between ranking, a workgroup's sort and sorting by launches."""
+    check_order(ids_of(torch.Generator().manual_seed(t + entries), t, entries, kind), entries)
+
+
 @pytest.mark.parametrize("count", [31, 32, 33, 63, 64, 65, 95, 96, 97, 128, 129])
 def test_ranges_around_a_chunk(torch_cuda, count):
     """Entries whose ranges begin and end at every place of a chunk."""

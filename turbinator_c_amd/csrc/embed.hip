@@ -120,6 +120,17 @@ __global__ __launch_bounds__(kThreads) void clear_kernel(i32x2 *ranges, size_t e
         ranges[v] = (i32x2){0, 0};
 }
 
+// The lanes with the same value of `bits` bits among those that are live.
+__device__ __forceinline__ unsigned long long same_lanes(bool live, unsigned value, int bits) {
+    unsigned long long same = __ballot(live);
+    for (int bit = 0; bit < bits; ++bit) {
+        const bool set = value >> bit & 1;
+        const unsigned long long all = __ballot(set);
+        same &= set ? all : ~all;
+    }
+    return same;
+}
+
 // Few tokens: a token's place is the number of smaller keys and of equal ones
 // before it, an entry's range what lies below and up to it.  Each lane has a
 // token (or an entry), each wave a share of the keys, which come through scalar
@@ -159,13 +170,7 @@ __global__ __launch_bounds__(64 * kRankWaves) void rank_kernel(OrderArgs a, unsi
         }
         if (tokens && j0 == i0) {
             // Behind the smaller ones, the lanes in front with the same key.
-            unsigned long long same = ~0ull;
-            for (int bit = 0; bit < a.bits; ++bit) {
-                const bool set = key >> bit & 1;
-                const unsigned long long all = __ballot(set);
-                same &= set ? all : ~all;
-            }
-            front += __popcll(same & ((1ull << lane) - 1));
+            front += __popcll(same_lanes(true, key, a.bits) & ((1ull << lane) - 1));
         }
         place += front;
     }
@@ -185,6 +190,89 @@ __global__ __launch_bounds__(64 * kRankWaves) void rank_kernel(OrderArgs a, unsi
         a.ranges[i] = most > less ? (i32x2){less, most} : (i32x2){0, 0};
     else if (RANGES && known && place == less)
         a.ranges[key] = (i32x2){less, most};
+}
+
+// Some thousand tokens: the counting sort below in one workgroup, keys and both
+// orders in LDS, seven bits or fewer at a time; tokens without an entry have the
+// largest key.  Each wave has a run of the order, of four turns at the most.
+constexpr int kSmallWaves = 16, kSmallSort = 64 * kSmallWaves, kSmallBits = 7;
+constexpr int kSmallTurns = 4;
+constexpr size_t kSmallMost = kSmallSort * kSmallTurns;
+
+__global__ __launch_bounds__(kSmallSort) void sort_kernel(OrderArgs a, int passes, bool clear) {
+    __shared__ unsigned key[kSmallMost];
+    __shared__ unsigned short order[2][kSmallMost];
+    __shared__ int next[kSmallWaves][1 << kSmallBits], start[1 << kSmallBits];
+    const int t = threadIdx.x, wave = t >> 6, lane = t & 63, n = (int)a.tokens;
+    const int digits = 1 << a.bits, run = (n + kSmallSort - 1) / kSmallSort * 64;
+    // At most 64 kSmallTurns: n is at most kSmallMost.
+    const int c0 = wave * run, c1 = c0 + run < n ? c0 + run : n;
+    for (int c = t; c < n; c += kSmallSort) {
+        key[c] = entry_of(a.ids, a.entries, c);
+        order[0][c] = (unsigned short)c;
+    }
+    if (clear)
+        for (size_t v = t; v < a.entries; v += kSmallSort) a.ranges[v] = (i32x2){0, 0};
+    for (int p = 0; p < passes; ++p) {
+        const unsigned short *from = order[p & 1];
+        unsigned short *to = order[(p + 1) & 1];
+        const int shift = p * a.bits;
+        for (int i = t; i < kSmallWaves * digits; i += kSmallSort) next[i / digits][i % digits] = 0;
+        __syncthreads();
+        unsigned token[kSmallTurns], digit[kSmallTurns];
+#pragma unroll
+        for (int j = 0; j < kSmallTurns; ++j)
+            token[j] = c0 + 64 * j + lane < c1 ? from[c0 + 64 * j + lane] : 0;
+#pragma unroll
+        for (int j = 0; j < kSmallTurns; ++j) {
+            digit[j] = key[token[j]] >> shift & (digits - 1);
+            if (c0 + 64 * j + lane < c1) atomicAdd(&next[wave][digit[j]], 1);
+        }
+        __syncthreads();
+        if (t < digits) {
+            int all = 0;
+            for (int w = 0; w < kSmallWaves; ++w) {
+                const int count = next[w][t];
+                next[w][t] = all;
+                all += count;
+            }
+            start[t] = all;
+        }
+        __syncthreads();
+        if (wave == 0) {
+            int below = 0;
+            for (int d0 = 0; d0 < digits; d0 += 64) {
+                const int d = d0 + lane, count = d < digits ? start[d] : 0;
+                const int sum = running_sum(count);
+                if (d < digits) start[d] = below + sum - count;
+                below += __builtin_amdgcn_readlane(sum, 63);
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < kSmallTurns; ++j) {
+            if (c0 + 64 * j >= c1) break;
+            const bool live = c0 + 64 * j + lane < c1;
+            const unsigned d = digit[j];
+            const unsigned long long same = same_lanes(live, d, a.bits);
+            const int rank = __popcll(same & ((1ull << lane) - 1));
+            const int at = next[wave][d] + rank;
+            wave_fence();
+            if (live && rank == 0) next[wave][d] = at + __popcll(same);
+            wave_fence();
+            if (live) to[start[d] + at] = (unsigned short)token[j];
+        }
+        __syncthreads();
+    }
+    const unsigned short *sorted = order[passes & 1];
+    for (int c = t; c < n; c += kSmallSort) {
+        const unsigned token = sorted[c], id = key[token];
+        const bool known = id < a.entries;
+        a.to[c] = known ? (int)token : -1;
+        int *range = reinterpret_cast<int *>(a.ranges + id);
+        if (known && (c == 0 || key[sorted[c - 1]] != id)) range[0] = c;
+        if (known && (c + 1 == n || key[sorted[c + 1]] != id)) range[1] = c + 1;
+    }
 }
 
 // Many tokens: a stable counting sort by digits, the least first; tokens
@@ -289,13 +377,7 @@ __global__ __launch_bounds__(kSortThreads) void place_kernel(OrderArgs a) {
         for (int j = 0; j < kBatch; ++j) {
             const unsigned d = now.digit[j];
             const bool live = d != ~0u;
-            // The lanes with the same digit.
-            unsigned long long same = __ballot(live);
-            for (int bit = 0; bit <= a.bits; ++bit) {
-                const bool set = d >> bit & 1;
-                const unsigned long long all = __ballot(set);
-                same &= set ? all : ~all;
-            }
+            const unsigned long long same = same_lanes(live, d, a.bits + 1);
             const int rank = __popcll(same & ((1ull << lane) - 1));
             int at = 0;
             if (live) at = next[d] + rank;
@@ -567,10 +649,12 @@ bool rows_ok(const void *p, size_t stride, int dtype) {
     return p && multiple_of(p, type_size(dtype)) && stride % type_size(dtype) == 0;
 }
 
-// Ranking takes tokens^2 comparisons, sorting up to five launches: 1,024 tokens
-// are ranked in 4.4 us, 6,000 in 17, with the gradient of 1,000 x 256 and the
-// launches 41 us, where sorting takes 34.
-constexpr size_t kRankMost = 4096, kRankEntries = 4096, kRankRanges = 2048;
+// Ranking takes tokens^2 comparisons, a workgroup's sort its own chain, sorting by
+// launches up to five of them.  Orders on the GPU: 1,024 tokens ranked 4.3 us,
+// 2,000 7.5; 3,000 to 4,096 sorted by one workgroup 7 to 9.  With the gradient of
+// 4,096 tokens to 100 entries and the launches: ranked 16.4 us, one workgroup
+// 14.0, by launches 17; of 6,000 tokens to 1,000: one workgroup 36, launches 34.
+constexpr size_t kRankMost = 2048, kRankEntries = 4096;
 
 int log2_up(size_t n) {
     int bits = 0;
@@ -718,23 +802,24 @@ extern "C" int tb_hip_embed_order_device(const int *ids, int *order, int *ranges
     auto clear = [&] {
         clear_kernel<<<grid_of(entries, kThreads), kThreads, 0, q>>>(a.ranges, entries);
     };
-    auto find_ranges = [&] {
-        range_kernel<<<grid_of(tokens, kThreads), kThreads, 0, q>>>(a);
-    };
+    const bool few_entries = entries <= kRankEntries;
     if (tokens <= kRankMost) {
         const unsigned blocks = (unsigned)((tokens + 63) / 64);
         a.bits = log2_up(entries + 1);
-        if (entries <= kRankEntries) {
+        if (few_entries) {
             const unsigned more = (unsigned)((entries + 63) / 64);
             rank_kernel<false><<<blocks + more, 64 * kRankWaves, 0, q>>>(a, blocks);
-        } else if (tokens <= kRankRanges) {
-            clear();
-            rank_kernel<true><<<blocks, 64 * kRankWaves, 0, q>>>(a, blocks);
         } else {
             clear();
-            rank_kernel<false><<<blocks, 64 * kRankWaves, 0, q>>>(a, blocks);
-            find_ranges();
+            rank_kernel<true><<<blocks, 64 * kRankWaves, 0, q>>>(a, blocks);
         }
+        return hipGetLastError() == hipSuccess;
+    }
+    if (tokens <= kSmallMost) {
+        const int bits = log2_up(entries + 1), passes = (bits + kSmallBits - 1) / kSmallBits;
+        a.bits = (bits + passes - 1) / passes;
+        if (!few_entries) clear();
+        sort_kernel<<<1, kSmallSort, 0, q>>>(a, passes, few_entries);
         return hipGetLastError() == hipSuccess;
     }
     const SortShape s = sort_shape(tokens, entries);
@@ -750,7 +835,7 @@ extern "C" int tb_hip_embed_order_device(const int *ids, int *order, int *ranges
     }
     a.last = 1;
     sort_pass(a, s.high ? s.low : 0, s.high ? s.high : s.low, q);
-    if (s.high) find_ranges();
+    if (s.high) range_kernel<<<grid_of(tokens, kThreads), kThreads, 0, q>>>(a);
     return hipGetLastError() == hipSuccess;
 }
 
