@@ -8,6 +8,11 @@
 //
 // The gradient adds rows up in the order's order, so that it never depends on
 // timing; every entry's row is written once, dout is read once.
+//
+// Lookup is bound by memory: 163,840 x 1,024 bf16 of 32,768 entries 92 us (84 at a
+// copy's rate).  The gradient of as much, skewed: the order 34 us, five launches
+// of which each is mostly its own chain; the sums 103 us for the 470 MB of dout
+// and table and 30 to 40 of parts (4.9 TB/s); the joins 14.
 #include "layer_math.h"
 
 namespace {

@@ -26,7 +26,9 @@ __host__ __device__ inline size_t padded(size_t k) { return (k + kPad - 1) / kPa
 // --------------------------------------------------------------------------
 // Quantisation: a row belongs to one wave or to a workgroup, eight values of a
 // lane at a time, kept in registers between the maximum and the codes where
-// they fit.
+// they fit.  Bound by memory: 40,959 x 1,999 bf16 54 us, the values back 37 us (4.6
+// and 6.7 TB/s of what they read and write, the codes in between in the last
+// cache); 16,384 x 4,096 bf16 41 us, 4.9 TB/s.
 
 constexpr int kQuantThreads = 256;
 
@@ -310,28 +312,6 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_kernel(ProductArgs a) {
     }
 }
 
-// Staged tiles of BM rows and BN columns: slices of two steps (128 values, 128
-// bytes a row) through STAGES buffers in LDS.
-//
-// Codes come by loads that write LDS themselves: a wave's load fills 1 KB,
-// eight rows, in lane order.  16-byte piece c of row r lies at slot c ^ (r & 7)
-// of its row, so that the rows of an operand read, 128 bytes apart, fall on
-// all banks.
-//
-// Turn s: wait for the loads of slice s + 1; barrier: all waves have them, and
-// have read slice s; then a step's products at a time, in NT groups, among them
-// the loads of slice s + STAGES over slice s and the reads of the next step.
-// The loads go early where the next turn waits for them (two buffers), else over
-// the whole turn; all of them in a row would hold up the wave's products.
-//
-// m 16,384, n 4,096, k 4,096: 217 to 241 us by the card, 2.3 to 2.5 PFLOP/s; the
-// instruction does 4.0 from registers, where the card's power holds its clock at
-// 1.9 GHz (2.1 here, the matrix units busy in 60% of the cycles).  Of the 60 us of
-// a round of 256 tiles the products take 32, LDS reads and barriers add 4, loads
-// 12 (8 out of the last cache), start, activation and stores 10: an operation on
-// every output costs 0.5 us, GELU 8.  Tried and not faster: slices of one step in
-// four buffers, three buffers under tiles of 128 rows, rows touched ahead to have
-// them in the L2.
 // 16 bytes of columns from n0 on of row r, past the caches: nothing here reads
 // them again (16,384 x 4,096 x 4,096: 232 us, with ordinary stores 250).
 template <class T>
@@ -404,6 +384,28 @@ __device__ __forceinline__ int spread_of(int row) {
     return (row & 3) | (row >> 3 & 1) << 2;
 }
 
+// Staged tiles of BM rows and BN columns: slices of two steps (128 values, 128
+// bytes a row) through STAGES buffers in LDS.
+//
+// Codes come by loads that write LDS themselves: a wave's load fills 1 KB,
+// eight rows, in lane order.  16-byte piece c of row r lies at slot c ^ (r & 7)
+// of its row (of a column: c ^ spread_of it), so that the rows of an operand
+// read, 128 bytes apart, fall on all banks.
+//
+// Turn s: wait for the loads of slice s + 1; barrier: all waves have them, and
+// have read slice s; then a step's products at a time, in NT groups, among them
+// the loads of slice s + STAGES over slice s and the reads of the next step.
+// The loads go early where the next turn waits for them (two buffers), else over
+// the whole turn; all of them in a row would hold up the wave's products.
+//
+// m 16,384, n 4,096, k 4,096: 217 to 241 us by the card, 2.3 to 2.5 POPS; the
+// instruction does 4.0 from registers, where the card's power holds its clock at
+// 1.9 GHz (2.1 here, the matrix units busy in 60% of the cycles).  Of the 60 us of
+// a round of 256 tiles the products take 32, LDS reads and barriers add 4, loads
+// 12 (8 out of the last cache), start, activation and stores 10: an operation on
+// every output costs 0.5 us, GELU 8.  Tried and not faster: slices of one step in
+// four buffers, three buffers under tiles of 128 rows, rows touched ahead to have
+// them in the L2.
 template <class T, int ACT, int WM, int WN, int MT, int NT, int STAGES>
 __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(ProductArgs a) {
     constexpr int BM = 16 * MT * WM, BN = 16 * NT * WN, kWaves = WM * WN, kThreads = 64 * kWaves;
@@ -488,8 +490,8 @@ __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(ProductArgs a) {
     };
     const int row_x = wm * MT * 16, row_w = BM + wn * NT * 16;
     const int lane_row = low * kPad, slot = (part ^ (low & 7)) * 16;
+    // The same slot for every column tile: they differ in bits that spread_of leaves out.
     const int w_row = column_of<T>(0, low), w_slot = (part ^ spread_of<T>(w_row)) * 16;
-    const int w_slot1 = (part ^ spread_of<T>(column_of<T>(1, low))) * 16;
     // Read `r` of a step's operands, the rows' first.
     auto read_one = [&](unsigned stage, int s, Operands<MT, NT> &o, int r) {
         if (r < MT) {
@@ -497,10 +499,9 @@ __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(ProductArgs a) {
             o.x[r] = *reinterpret_cast<const i32x4 *>(p + (row_x + r * 16) * kPad);
         } else {
             const int i = r - MT;
-            const unsigned char *p = codes + stage + w_row * kPad +
-                                     ((i % 2 ? w_slot1 : w_slot) ^ (s * kStep));
-            o.w[i] = *reinterpret_cast<const i32x4 *>(
-                p + (row_w + column_of<T>(i, 0)) * kPad);
+            const unsigned char *p = codes + stage + w_row * kPad + (w_slot ^ (s * kStep));
+            o.w[i] =
+                *reinterpret_cast<const i32x4 *>(p + (row_w + column_of<T>(i, 0)) * kPad);
         }
     };
     Operands<MT, NT> even, odd;
@@ -708,8 +709,8 @@ static_assert(64 * kFewWaves * (size_t)kGridRow < size_t(1) << 32);
 //   m     64 n 4,096 k 1,024: 6.3 (low) / 5.3 / 7.1
 //   m     32 n 4,096 k 4,096: 13.1 (low) / 10.0 / 10.7
 //   m     16 n 4,096 k 4,096: 12.8 (low) / 10.0 / 7.6
-// The cheapest by the costs above, which chooses the fastest in every line but
-// the experts' few; within 6% of it elsewhere in the range measured.
+// The cheapest by the costs above: the fastest in every line, or within 2% of it;
+// elsewhere within 7% (12,000 x 1,500 x 700: 32 us in middle tiles, 30 in high).
 int shape_for(const ProductArgs &a) {
     // The staged kernels count a matrix in 32 bits of 16 bytes, from a tile's
     // first row (from the first of all where rows are gathered).
