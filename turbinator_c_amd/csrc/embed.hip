@@ -10,9 +10,9 @@
 // timing; every entry's row is written once, dout is read once.
 //
 // Lookup is bound by memory: 163,840 x 1,024 bf16 of 32,768 entries 92 us (84 at a
-// copy's rate).  The gradient of as much, skewed: the order 34 us, five launches
-// of which each is mostly its own chain; the sums 103 us for the 470 MB of dout
-// and table and 30 to 40 of parts (4.9 TB/s); the joins 14.
+// copy's rate).  The gradient of as much, skewed: the order 35 us, five launches
+// of which each is mostly its own chain; the sums 86 us for the 470 MB of dout
+// and table and 30 to 40 of parts (5.9 TB/s); the joins 15.
 #include "layer_math.h"
 
 namespace {
@@ -284,7 +284,7 @@ __global__ __launch_bounds__(kSmallSort) void sort_kernel(OrderArgs a, int passe
 // without an entry have a digit of their own behind the others.  A workgroup
 // has a segment of the tokens, each of its waves a run of it.
 constexpr int kSortWaves = 8, kSortThreads = 64 * kSortWaves;
-constexpr size_t kSegment = 2048, kMaxSegments = 256;
+constexpr size_t kSegment = 1024, kMaxSegments = 256;
 
 __device__ __forceinline__ unsigned digit_of(const OrderArgs &a, size_t c, int &token) {
     token = a.from ? a.from[c] : (int)c;
@@ -445,26 +445,33 @@ __device__ __forceinline__ long long entry_at(const GradArgs &a, size_t place) {
 }
 
 // Adds up element e on of the rows at every `step`th place from b to end of the
-// order, four rows at a time and those in pairs.  More at a time cost registers,
-// and with them waves whose chains of loads (range, places, rows) overlap:
-// 163,840 x 1,024 bf16 to 32,768 entries with their order 162 us, and 166 with
-// two, 183 with eight, 242 with sixteen.
+// order, four rows at a time and those in pairs, the next places on their way
+// meanwhile.  More at a time cost registers, and with them waves whose chains of
+// loads (range, places, rows) overlap: 163,840 x 1,024 bf16 to 32,768 entries
+// with their order 137 us, and 142 with two, 149 with eight (153 without looking
+// ahead); of smaller gradients eight would save up to 8%.
 template <class T, int B, bool STREAM>
 __device__ __forceinline__ void add_rows(const GradArgs &a, long long b, long long end, int step,
                                          unsigned e, float (&sum)[Vec<T, B>::n]) {
     typedef Vec<T, B> X;
     constexpr int kAhead = 4;
+    int token[kAhead];
+    auto look = [&](long long first) {
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i)
+            token[i] = first + i * step < end ? a.order[first + i * step] : -1;
+    };
+    look(b);
     for (; b < end; b += kAhead * step) {
         typename X::raw row[kAhead];
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) {
-            const long long at = b + i * step;
-            const int t = at < end ? a.order[at] : -1;
-            const char *from = a.dout + (size_t)t * a.stride;
+            const char *from = a.dout + (size_t)token[i] * a.stride;
             row[i] = typename X::raw{};
-            if (t >= 0 && (size_t)t < a.tokens)
+            if (token[i] >= 0 && (size_t)token[i] < a.tokens)
                 row[i] = STREAM ? stream_in<T, B>(from, e) : load_loose<T, B>(from, e);
         }
+        look(b + kAhead * step);  // on their way with the rows
         float x[kAhead][X::n];
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) X::unpack(row[i], x[i]);
@@ -545,8 +552,8 @@ __global__ __launch_bounds__(kThreads) void grad_kernel(GradArgs a) {
 // and finds the ranges that start in its chunks, at most one in each.  Those of
 // a few parts are added up by 16 lanes each, the others by the workgroup.  More
 // threads would shorten a single range's chain (163,840 tokens of one entry,
-// 512 wide, with their order 73 us, with 512 threads 67), but most workgroups
-// find little to do (32,768 entries, 1,024 wide: 153 and 161 us).
+// 512 wide, with their order 6 of 73 us with 512 threads), but most workgroups
+// find little to do (32,768 entries, 1,024 wide: 8 of 153 us more).
 constexpr int kJoinThreads = 256, kJoinLanes = 16, kJoinGroups = kJoinThreads / kJoinLanes;
 constexpr int kJoinColumns = 4 * kJoinLanes, kJoinChunks = 16, kJoinShort = 8;
 static_assert(kJoinChunks <= kJoinGroups);
@@ -658,7 +665,7 @@ bool rows_ok(const void *p, size_t stride, int dtype) {
 // launches up to five of them.  Orders on the GPU: 1,024 tokens ranked 4.3 us,
 // 2,000 7.5; 3,000 to 4,096 sorted by one workgroup 7 to 9.  With the gradient of
 // 4,096 tokens to 100 entries and the launches: ranked 16.4 us, one workgroup
-// 14.0, by launches 17; of 6,000 tokens to 1,000: one workgroup 36, launches 34.
+// 14.0, by launches 17; of 6,000 tokens to 1,000: one workgroup 2 us more.
 constexpr size_t kRankMost = 2048, kRankEntries = 4096;
 
 int log2_up(size_t n) {
