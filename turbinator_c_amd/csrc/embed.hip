@@ -10,7 +10,7 @@
 // timing; every entry's row is written once, dout is read once.
 //
 // Lookup is bound by memory: 163,840 x 1,024 bf16 of 32,768 entries 92 us (84 at a
-// copy's rate).  The gradient of as much, skewed: the order 35 us, five launches
+// copy's rate).  The gradient of as much, skewed: the order 32 us, five launches
 // of which each is mostly its own chain; the sums 86 us for the 470 MB of dout
 // and table and 30 to 40 of parts (5.9 TB/s); the joins 15.
 #include "layer_math.h"
@@ -282,9 +282,12 @@ __global__ __launch_bounds__(kSmallSort) void sort_kernel(OrderArgs a, int passe
 
 // Many tokens: a stable counting sort by digits, the least first; tokens
 // without an entry have a digit of their own behind the others.  A workgroup
-// has a segment of the tokens, each of its waves a run of it.
-constexpr int kSortWaves = 8, kSortThreads = 64 * kSortWaves;
-constexpr size_t kSegment = 1024, kMaxSegments = 256;
+// has a segment of the tokens, each of its waves a run of it.  Segments of 512:
+// 12,693 tokens to 2,945 x 592 fp16 with their gradient 35.5 us, of 1,024 37.2;
+// more than 256 of them make every workgroup add up more counts than it places
+// tokens (163,840 tokens: 135 us with 256 at the most, 146 with 320).
+constexpr int kSortBits = 9, kSortThreads = 1 << kSortBits, kSortWaves = kSortThreads / 64;
+constexpr size_t kSegment = 512, kMaxSegments = 256;
 
 __device__ __forceinline__ unsigned digit_of(const OrderArgs &a, size_t c, int &token) {
     token = a.from ? a.from[c] : (int)c;
@@ -314,40 +317,77 @@ __global__ __launch_bounds__(kSortThreads) void count_kernel(OrderArgs a) {
 }
 
 // A lane's tokens of one turn and their digits, one past the others behind c1.
-constexpr int kBatch = 4;
+constexpr int kBatch = 4, kCounts = 16;
 struct Turn {
-    int token[kBatch];
+    int token[kBatch];  // -1 behind c1
     unsigned digit[kBatch];
-    __device__ __forceinline__ void load(const OrderArgs &a, size_t c, size_t c1) {
+    __device__ __forceinline__ void tokens(const OrderArgs &a, size_t c, size_t c1) {
 #pragma unroll
         for (int j = 0; j < kBatch; ++j) {
-            digit[j] = ~0u;
-            if (c + 64 * j < c1) digit[j] = digit_of(a, c + 64 * j, token[j]);
+            const size_t at = c + 64 * j;
+            token[j] = at >= c1 ? -1 : a.from ? a.from[at] : (int)at;
         }
+    }
+    __device__ __forceinline__ void keys(const OrderArgs &a) {
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) digit[j] = (unsigned)a.ids[token[j] < 0 ? 0 : token[j]];
+    }
+    __device__ __forceinline__ void digits(const OrderArgs &a) {
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j)
+            digit[j] = token[j] < 0              ? ~0u
+                       : digit[j] < a.entries ? digit[j] >> a.shift & ((1u << a.bits) - 1)
+                                              : 1u << a.bits;
+    }
+    __device__ __forceinline__ void load(const OrderArgs &a, size_t c, size_t c1) {
+        tokens(a, c, c1);
+        keys(a);
+        digits(a);
     }
 };
 
 __global__ __launch_bounds__(kSortThreads) void place_kernel(OrderArgs a) {
     extern __shared__ int lds[];
-    const int digits = (1 << a.bits) + 1, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    int *start = lds, *next = lds + digits * (1 + wave);
-    for (int i = threadIdx.x; i < digits * kSortWaves; i += kSortThreads) lds[digits + i] = 0;
+    const int digits = (1 << a.bits) + 1, lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    int *start = lds, *next = lds + digits * (1 + wave), *before = lds + digits * (1 + kSortWaves);
     const size_t run = a.segment / kSortWaves, c0 = blockIdx.x * a.segment + wave * run;
     const size_t c1 = c0 + run < a.tokens ? c0 + run : a.tokens;
     Turn now;
-    now.load(a, c0 + lane, c1);
-    // Of each digit: all segments' counts, and those of the segments before.
-    for (int d = threadIdx.x; d < digits; d += kSortThreads) {
-        int all = 0, before = 0;
-#pragma unroll 16
-        for (unsigned s = 0; s < a.segments; ++s) {
-            const int n = a.counts[(size_t)s * digits + d];
-            all += n;
-            before += s < blockIdx.x ? n : 0;
+    now.tokens(a, c0 + lane, c1);
+    for (int i = threadIdx.x; i < digits * (2 + kSortWaves); i += kSortThreads) lds[i] = 0;
+    __syncthreads();
+    now.keys(a);
+    // The last digit needs the counts before only: nothing lies behind it.
+    static_assert(kMaxSegments <= kSortThreads);
+    int none = 0;
+    if (threadIdx.x < blockIdx.x) none = a.counts[(size_t)threadIdx.x * digits + digits - 1];
+    // Of the others: all segments' counts, and those of the segments before.  The
+    // segments are shared out, and a thread's counts of kCounts are on their way
+    // at once.
+    const int shares = a.bits < kSortBits ? 1 << (kSortBits - a.bits) : 1;
+    for (int i = threadIdx.x; i < shares << a.bits; i += kSortThreads) {
+        const int d = i & ((1 << a.bits) - 1);
+        int all = 0, front = 0;
+        for (unsigned s0 = i >> a.bits; s0 < a.segments; s0 += shares * kCounts) {
+            int n[kCounts];
+#pragma unroll
+            for (int j = 0; j < kCounts; ++j) {
+                const unsigned s = s0 + j * shares;
+                n[j] = a.counts[(s < a.segments ? s : 0u) * digits + d];
+            }
+#pragma unroll
+            for (int j = 0; j < kCounts; ++j) {
+                const unsigned s = s0 + j * shares;
+                all += s < a.segments ? n[j] : 0;
+                front += s < blockIdx.x ? n[j] : 0;
+            }
         }
-        start[d] = all;
-        lds[digits * (1 + kSortWaves) + d] = before;
+        atomicAdd(&start[d], all);
+        atomicAdd(&before[d], front);
     }
+    if (none) atomicAdd(&before[digits - 1], none);
+    now.digits(a);
     __syncthreads();
     for (size_t c = c0; c < c1; c += 64 * kBatch) {
         if (c > c0) now.load(a, c + lane, c1);
@@ -359,7 +399,7 @@ __global__ __launch_bounds__(kSortThreads) void place_kernel(OrderArgs a) {
         int below = 0;
         for (int d0 = 0; d0 < digits; d0 += 64) {
             const int d = d0 + lane, n = d < digits ? start[d] : 0, sum = running_sum(n);
-            if (d < digits) start[d] = below + sum - n + lds[digits * (1 + kSortWaves) + d];
+            if (d < digits) start[d] = below + sum - n + before[d];
             if (a.last && !a.shift && blockIdx.x == 0 && (size_t)d < a.entries)
                 a.ranges[d] = n ? (i32x2){below + sum - n, below + sum} : (i32x2){0, 0};
             below += __builtin_amdgcn_readlane(sum, 63);
@@ -380,6 +420,7 @@ __global__ __launch_bounds__(kSortThreads) void place_kernel(OrderArgs a) {
         if (run > 64 * kBatch) now.load(a, c + lane, c1);
 #pragma unroll
         for (int j = 0; j < kBatch; ++j) {
+            if (c + 64 * j >= c1) break;
             const unsigned d = now.digit[j];
             const bool live = d != ~0u;
             const unsigned long long same = same_lanes(live, d, a.bits + 1);
@@ -449,7 +490,7 @@ __device__ __forceinline__ long long entry_at(const GradArgs &a, size_t place) {
 // meanwhile.  More at a time cost registers, and with them waves whose chains of
 // loads (range, places, rows) overlap: 163,840 x 1,024 bf16 to 32,768 entries
 // with their order 137 us, and 142 with two, 149 with eight (153 without looking
-// ahead); of smaller gradients eight would save up to 8%.
+// ahead); of smaller gradients eight saves up to 8%.
 template <class T, int B, bool STREAM>
 __device__ __forceinline__ void add_rows(const GradArgs &a, long long b, long long end, int step,
                                          unsigned e, float (&sum)[Vec<T, B>::n]) {
@@ -663,9 +704,10 @@ bool rows_ok(const void *p, size_t stride, int dtype) {
 
 // Ranking takes tokens^2 comparisons, a workgroup's sort its own chain, sorting by
 // launches up to five of them.  Orders on the GPU: 1,024 tokens ranked 4.3 us,
-// 2,000 7.5; 3,000 to 4,096 sorted by one workgroup 7 to 9.  With the gradient of
-// 4,096 tokens to 100 entries and the launches: ranked 16.4 us, one workgroup
-// 14.0, by launches 17; of 6,000 tokens to 1,000: one workgroup 2 us more.
+// 2,000 7.5; 3,000 to 4,096 sorted by one workgroup 7 to 9.  With their gradient
+// and the launches, one workgroup and by launches: 2,100 tokens to 1,000 entries
+// 15.1 and 18.0 us, 4,096 tokens 19.3 and 19.5, 6,000 tokens 36 and 28; 4,096
+// ranked take 2 us more than sorted.
 constexpr size_t kRankMost = 2048, kRankEntries = 4096;
 
 int log2_up(size_t n) {
