@@ -225,6 +225,22 @@ def test_infinities_stay_in_their_entry(torch_cuda):
     assert got.isfinite().all()
 
 
+@pytest.mark.parametrize("t", [500, 9000])
+def test_ranges_past_the_order_hold_nothing(torch_cuda, t):
+    """Ranges that start behind the last place, up to the largest: no tokens."""
+    g = torch.Generator().manual_seed(9)
+    ids = ids_of(g, t, 40, "even")
+    order, ranges = check_order(ids, 40)
+    dout = spread(g, t, 40, torch.float32)
+    want = backward(ids.cuda(), order, ranges, dout, 1.0, 40)
+    most = 2 ** 31 - 1
+    ranges[3], ranges[17], ranges[39] = (torch.tensor(r, dtype=torch.int32)
+                                         for r in ((most, most), (most - 9, most), (t, most)))
+    for entry in (3, 17, 39):
+        want[entry] = 0
+    assert torch.equal(backward(ids.cuda(), order, ranges, dout, 1.0, 40), want)
+
+
 def test_gradient_by_differences(torch_cuda):
     """The lookup is linear in the table: central differences are exact but for
     the roundings of the outputs (u of 2 * 4.5 + 4.5 each, times a gradient of

@@ -696,7 +696,7 @@ __global__ __launch_bounds__(kSmallThreads) void small_kernel(GradArgs a) {
     const unsigned e = there ? first_of<N>(a.s, v) : 0;
     const i32x2 r = range_of(a, entry);
     float sum[N] = {};
-    if (there) add_rows<T, B, false>(a, r[0] + (int)group, r[1], groups, e, sum);
+    if (there) add_rows<T, B, false>(a, (long long)r[0] + group, r[1], groups, e, sum);
     const unsigned used = r[1] - r[0] < (int)groups ? r[1] > r[0] ? r[1] - r[0] : 0 : groups;
     unsigned half = 1;
     while (half < used) half *= 2;
