@@ -333,11 +333,10 @@ __device__ __forceinline__ void store_columns(const ProductArgs &a, size_t r, si
 // 16 bytes of each lane to 1 KB of LDS from `to` on.  In assembly, because the
 // compiler, which follows such loads in LDS, waits for all of them before it
 // reads any LDS behind a loop's start, the ones just issued too: the waits are
-// arrive_but's.  m0 holds the place in LDS; nothing else here uses it.
+// arrive_but's.  The place in LDS stands in m0, as an operand: the compiler
+// writes it and knows what it holds; the pause behind that write is needed.
 __device__ __forceinline__ void fetch(const void *from, unsigned to) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to),
-                 "v"(from)
-                 : "memory");
+    asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"{m0}"(to), "v"(from) : "memory");
 }
 
 // Waits for all but the wave's last `COUNT` loads and for its LDS accesses, then
