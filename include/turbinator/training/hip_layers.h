@@ -154,8 +154,16 @@ size_t tb_hip_expert_order_workspace_bytes(size_t tokens, int n_experts, int k);
  * are strided (a stride may be 0), outputs dense, all of one type, at any
  * element.  Sums run over j in order, in 32 bits, and are rounded once.
  *
- * rows[p] = w x[t]; the rows from offsets[n_experts] on are 0, and a choice
- * whose position lies there has none.  Without weights rows are copied as they
+ * Positions and offsets belong together: in the order's, every choice with a
+ * row has it below offsets[n_experts], and the others are -1.  The two entries
+ * that write rows clear those from offsets[n_experts] on, and take a position
+ * there as none; the two that read rows do not know offsets and read the row of
+ * any position below tokens * k.  So who lowers offsets[n_experts] sets the
+ * positions from there on to -1: otherwise the gradients below are not those of
+ * the entries before them.
+ *
+ * rows[p] = w x[t]; the rows from offsets[n_experts] on are 0, others that no
+ * choice has are left as they were.  Without weights rows are copied as they
  * are.  Two choices must not have the same row. */
 int tb_hip_expert_rows_device(const void *x, size_t row_stride, const int *offsets,
                               const int *positions, const float *weights, void *rows,
@@ -180,7 +188,9 @@ int tb_hip_expert_sum_device(const void *rows, size_t row_stride, const int *pos
 
 /* Its gradients: drows[p] = w dout[t], 0 from offsets[n_experts] on as above,
  * and, unless dweights is NULL, dweights[t, j] = the product of rows[p] and
- * dout[t].  rows is read for dweights only.  The residual's gradient is dout.
+ * dout[t] (0 for a choice without a row, and for one whose position lies from
+ * offsets[n_experts] on).  rows is read for dweights only.  The residual's
+ * gradient is dout.
  *
  * The four return 0 for NULL pointers that are not said to be nullable, tokens
  * 0 or tokens * k above 0x7fffffff, n_experts outside

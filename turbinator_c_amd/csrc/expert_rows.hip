@@ -44,7 +44,9 @@ constexpr bool has_dots(int kind) { return kind >= kRowsBack && kind != kSum; }
 // each, summed in 300 us, and in 332 with room for eight.
 constexpr int kFew = 2, kSome = 4, kMost = 8;
 
-// A choice's row, -1 for none.
+// A choice's row, -1 for none.  `end` is one behind the last expert's rows where
+// the entry has offsets, else of all rows: positions from the former on are the
+// caller's to set to -1, for the gradients' sake.
 __device__ __forceinline__ long long row_of(const TokenArgs &a, size_t choice, size_t end) {
     const int p = a.positions[choice];
     return p >= 0 && (size_t)p < end ? p : -1;
