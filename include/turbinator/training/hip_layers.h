@@ -227,9 +227,11 @@ int tb_hip_embed_order_device(const int *ids, int *order, int *ranges, void *wor
 size_t tb_hip_embed_order_workspace_bytes(size_t tokens, size_t entries);
 
 /* dtable[v] = scale * the sum of dout[t] over the tokens with ids[t] = v, in
- * the order's order and in 32 bits ([entries, width] fp32, dense; rows of
- * entries without tokens are 0).  dout is strided (the stride may be 0); rows
- * of tokens without an entry are not read.  order and ranges as
+ * 32 bits ([entries, width] fp32, dense; rows of entries without tokens are 0).
+ * Partial sums are joined in a way that order, ranges and the sizes fix: the
+ * same on every call with the same arguments, but an entry's sum may round
+ * otherwise among other tokens or entries.  dout is strided (the stride may be
+ * 0); rows of tokens without an entry are not read.  order and ranges as
  * tb_hip_embed_order_device gives them for these ids.
  * workspace: tb_hip_embed_backward_workspace_bytes(...) bytes, 16-byte aligned;
  * it may be the order's, which is done with.

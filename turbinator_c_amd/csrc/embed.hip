@@ -6,8 +6,10 @@
 //              range v = the places of entry v's tokens in it
 //   gradient   dtable[v] = scale sum_{t: id[t] = v} dout[t]
 //
-// The gradient adds rows up in the order's order, so that it never depends on
-// timing; every entry's row is written once, dout is read once.
+// The gradient adds up partial sums of the order's places, whose tree the ranges
+// and sizes fix, so that it never depends on timing (but on where a range lies
+// among the chunks, and on the kernel that the sizes choose); every entry's row
+// is written once, dout is read once.
 //
 // Lookup is bound by memory: 163,840 x 1,024 bf16 of 32,768 entries 92 us (84 at a
 // copy's rate).  The gradient of as much, skewed: the order 32 us, five launches
