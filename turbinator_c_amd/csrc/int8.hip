@@ -397,14 +397,14 @@ __device__ __forceinline__ int spread_of(int row) {
 // The loads go early where the next turn waits for them (two buffers), else over
 // the whole turn; all of them in a row would hold up the wave's products.
 //
-// m 16,384, n 4,096, k 4,096: 217 to 241 us by the card, 2.3 to 2.5 POPS; the
-// instruction does 4.0 from registers, where the card's power holds its clock at
-// 1.9 GHz (2.1 here, the matrix units busy in 60% of the cycles).  Of the 60 us of
-// a round of 256 tiles the products take 32, LDS reads and barriers add 4, loads
-// 12 (8 out of the last cache), start, activation and stores 10: an operation on
-// every output costs 0.5 us, GELU 8.  Tried and not faster: slices of one step in
-// four buffers, three buffers under tiles of 128 rows, rows touched ahead to have
-// them in the L2.
+// m 16,384, n 4,096, k 4,096: 212 to 241 us by the card, 2.3 to 2.6 POPS; the
+// instruction does 4.0 from registers, at 1.9 GHz.  By counters the matrix units
+// are busy in 64% of the cycles (55% with GELU, 72% at k 8,192), at 1.95 GHz (1.76
+// at k 8,192, of 2.4).  Between k 4,096 and 8,192, in the loop alone, they are in
+// 81%: of the 53 us of a round of 256 tiles the products take 34, the loop's waits
+// for loads, LDS and barriers 8, start and stores 11; GELU adds 8.  Tried and not
+// faster: slices of one step in four buffers, three buffers under tiles of 128
+// rows, rows touched ahead to have them in the L2.
 template <class T, int ACT, int WM, int WN, int MT, int NT, int STAGES>
 __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(ProductArgs a) {
     constexpr int BM = 16 * MT * WM, BN = 16 * NT * WN, kWaves = WM * WN, kThreads = 64 * kWaves;

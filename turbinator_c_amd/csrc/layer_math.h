@@ -58,11 +58,11 @@ __device__ __forceinline__ void store_loose(char *row, size_t element, typename 
     *reinterpret_cast<Loose<T, B> *>(row + element * sizeof(T)) = v;
 }
 
-// The same past the caches, for what is used once.  Loads go that way from
-// kStreamBytes on: less than that, or much of it, is still in the last cache
-// (256 MB) when it was written just before.  Rows of 1,024 bf16, two to a token,
-// summed: 20,000 rows 17.0 us past the caches and 14.6 through them, 60,000 rows
-// 43 and 46.
+// The same past the caches, for what is used once.  Loads for which a kernel has
+// that form go so from kStreamBytes on: less than that, or much of it, is still in
+// the last cache (256 MB) when it was written just before.  Rows of 1,024 bf16,
+// two to a token, summed: 20,000 rows 17.0 us past the caches and 14.6 through
+// them, 60,000 rows 43 and 46.
 constexpr size_t kStreamBytes = size_t(64) << 20;
 template <class T, int B>
 __device__ __forceinline__ typename Raw<B>::type stream_in(const char *row, size_t element) {
