@@ -196,7 +196,7 @@ int tb_hip_expert_sum_device(const void *rows, size_t row_stride, const int *pos
  * 0 or tokens * k above 0x7fffffff, n_experts outside
  * 1..TB_HIP_ROUTE_MAX_EXPERTS, k outside 1..TB_HIP_ROUTE_MAX_K, width 0 or
  * above 0x7fffffff, an unknown dtype, pointers or strides off the element's
- * size. */
+ * size (pointers to int and float off 4 bytes). */
 int tb_hip_expert_sum_backward_device(const void *dout, size_t dout_stride, const void *rows,
                                       size_t row_stride, const int *offsets,
                                       const int *positions, const float *weights, void *drows,
@@ -209,7 +209,7 @@ int tb_hip_expert_sum_backward_device(const void *dout, size_t dout_stride, cons
  * base are strided (a stride may be 0), out is dense.
  * Returns 0 for other NULL pointers, tokens 0 or above 0x7fffffff, entries
  * outside 1..TB_HIP_EMBED_MAX_ENTRIES, width 0 or above 0x7fffffff, an unknown
- * dtype, pointers or strides off the element's size. */
+ * dtype, pointers or strides off the element's size (ids off 4 bytes). */
 int tb_hip_embed_device(const int *ids, const void *table, size_t table_stride, const void *base,
                         size_t base_stride, float scale, void *out, size_t tokens,
                         size_t entries, size_t width, int dtype, void *stream);
@@ -221,7 +221,8 @@ int tb_hip_embed_device(const int *ids, const void *table, size_t table_stride, 
  *                        ranges[v, 1] - 1; both 0 for an entry without tokens
  * One order serves every gradient of these ids.  ranges must be 8-byte aligned.
  * workspace: tb_hip_embed_order_workspace_bytes(...) bytes, 16-byte aligned.
- * Returns 0 for NULL pointers, sizes as above, misaligned ranges or workspace. */
+ * Returns 0 for NULL pointers, sizes as above, ids or order off 4 bytes,
+ * misaligned ranges or workspace. */
 int tb_hip_embed_order_device(const int *ids, int *order, int *ranges, void *workspace,
                               size_t tokens, size_t entries, void *stream);
 size_t tb_hip_embed_order_workspace_bytes(size_t tokens, size_t entries);

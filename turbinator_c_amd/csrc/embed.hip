@@ -834,8 +834,8 @@ extern "C" int tb_hip_embed_device(const int *ids, const void *table, size_t tab
                                    const void *base, size_t base_stride, float scale, void *out,
                                    size_t tokens, size_t entries, size_t width, int dtype,
                                    void *stream) {
-    if (!ids || !sizes_ok(tokens, entries) || !width || width > kMaxCount || !known_type(dtype) ||
-        !rows_ok(table, table_stride, dtype) || !rows_ok(out, 0, dtype) ||
+    if (!ids || !words_ok(ids) || !sizes_ok(tokens, entries) || !width || width > kMaxCount ||
+        !known_type(dtype) || !rows_ok(table, table_stride, dtype) || !rows_ok(out, 0, dtype) ||
         (base && !rows_ok(base, base_stride, dtype)))
         return 0;
     LookupArgs a = {};
@@ -865,8 +865,8 @@ extern "C" size_t tb_hip_embed_order_workspace_bytes(size_t tokens, size_t entri
 
 extern "C" int tb_hip_embed_order_device(const int *ids, int *order, int *ranges, void *workspace,
                                          size_t tokens, size_t entries, void *stream) {
-    if (!ids || !order || !ranges || !multiple_of(ranges, 8) || !workspace ||
-        !multiple_of(workspace, 16) || !sizes_ok(tokens, entries))
+    if (!ids || !order || !words_ok(ids, order) || !ranges || !multiple_of(ranges, 8) ||
+        !workspace || !multiple_of(workspace, 16) || !sizes_ok(tokens, entries))
         return 0;
     OrderArgs a = {};
     a.ids = ids;
@@ -928,7 +928,7 @@ extern "C" int tb_hip_embed_backward_device(const void *dout, size_t dout_stride
                                             size_t entries, size_t width, int dtype,
                                             void *stream) {
     if (!ids || !order || !ranges || !multiple_of(ranges, 8) || !dtable ||
-        !multiple_of(dtable, 4) || !workspace || !multiple_of(workspace, 16) ||
+        !words_ok(ids, order, dtable) || !workspace || !multiple_of(workspace, 16) ||
         !sizes_ok(tokens, entries) || !width || width > kMaxCount || !known_type(dtype) ||
         !rows_ok(dout, dout_stride, dtype))
         return 0;

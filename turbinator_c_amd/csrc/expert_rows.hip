@@ -273,7 +273,8 @@ extern "C" int tb_hip_expert_rows_device(const void *x, size_t row_stride, const
                                          int dtype, void *stream) {
     if (!sizes_ok(tokens, k, width, dtype) || n_experts < 1 ||
         n_experts > TB_HIP_ROUTE_MAX_EXPERTS || !offsets || !positions ||
-        !rows_ok(x, row_stride, dtype) || !rows_ok(rows, 0, dtype))
+        !words_ok(offsets, positions, weights) || !rows_ok(x, row_stride, dtype) ||
+        !rows_ok(rows, 0, dtype))
         return 0;
     TokenArgs a = args_of(positions, weights, tokens, k, width);
     a.token_in = static_cast<const char *>(x);
@@ -288,8 +289,9 @@ extern "C" int tb_hip_expert_rows_backward_device(const void *drows, size_t drow
                                                   const int *positions, const float *weights,
                                                   void *dx, float *dweights, size_t tokens, int k,
                                                   size_t width, int dtype, void *stream) {
-    if (!sizes_ok(tokens, k, width, dtype) || !positions || !rows_ok(drows, drow_stride, dtype) ||
-        !rows_ok(dx, 0, dtype) || (dweights && (!multiple_of(dweights, 4) || !rows_ok(x, row_stride, dtype))))
+    if (!sizes_ok(tokens, k, width, dtype) || !positions ||
+        !words_ok(positions, weights, dweights) || !rows_ok(drows, drow_stride, dtype) ||
+        !rows_ok(dx, 0, dtype) || (dweights && !rows_ok(x, row_stride, dtype)))
         return 0;
     TokenArgs a = args_of(positions, weights, tokens, k, width);
     a.rows_in = static_cast<const char *>(drows);
@@ -308,8 +310,9 @@ extern "C" int tb_hip_expert_sum_device(const void *rows, size_t row_stride, con
                                         const float *weights, const void *residual,
                                         size_t residual_stride, void *out, size_t tokens, int k,
                                         size_t width, int dtype, void *stream) {
-    if (!sizes_ok(tokens, k, width, dtype) || !positions || !rows_ok(rows, row_stride, dtype) ||
-        !rows_ok(out, 0, dtype) || (residual && !rows_ok(residual, residual_stride, dtype)))
+    if (!sizes_ok(tokens, k, width, dtype) || !positions || !words_ok(positions, weights) ||
+        !rows_ok(rows, row_stride, dtype) || !rows_ok(out, 0, dtype) ||
+        (residual && !rows_ok(residual, residual_stride, dtype)))
         return 0;
     TokenArgs a = args_of(positions, weights, tokens, k, width);
     a.rows_in = static_cast<const char *>(rows);
@@ -328,8 +331,8 @@ extern "C" int tb_hip_expert_sum_backward_device(const void *dout, size_t dout_s
                                                  int k, size_t width, int dtype, void *stream) {
     if (!sizes_ok(tokens, k, width, dtype) || n_experts < 1 ||
         n_experts > TB_HIP_ROUTE_MAX_EXPERTS || !offsets || !positions ||
-        !rows_ok(dout, dout_stride, dtype) || !rows_ok(drows, 0, dtype) ||
-        (dweights && (!multiple_of(dweights, 4) || !rows_ok(rows, row_stride, dtype))))
+        !words_ok(offsets, positions, weights, dweights) || !rows_ok(dout, dout_stride, dtype) ||
+        !rows_ok(drows, 0, dtype) || (dweights && !rows_ok(rows, row_stride, dtype)))
         return 0;
     TokenArgs a = args_of(positions, weights, tokens, k, width);
     a.token_in = static_cast<const char *>(dout);

@@ -848,7 +848,7 @@ extern "C" int tb_hip_int8_product_device(const void *a_codes, const float *a_sc
         experts > TB_HIP_ROUTE_MAX_EXPERTS || (experts > 1 && !offsets) ||
         n > kMaxCount / experts || m > kMaxOutputs / n || (!rows && m != a_rows) ||
         !known_act(act) || !multiple_of(a_codes, 16) || !multiple_of(w_codes, 16) ||
-        !multiple_of(a_scales, 4) || !multiple_of(w_scales, 4) ||
+        !words_ok(a_scales, w_scales, rows, offsets, bias, row_scale) ||
         !multiple_of(out, type_size(dtype)))
         return 0;
     ProductArgs a = {};

@@ -204,5 +204,11 @@ inline bool known_type(int dtype) {
 }
 inline bool known_act(int act) { return act >= TB_HIP_ACT_NONE && act <= TB_HIP_ACT_GELU; }
 inline bool multiple_of(const void *p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+// 32-bit values at pointers that may be NULL: uniform loads leave out an
+// address's low two bits.
+template <class... P>
+bool words_ok(P *...p) {
+    return (multiple_of(p, 4) && ...);
+}
 
 }  // namespace layer
