@@ -10,9 +10,9 @@ from typing import NamedTuple
 
 from turbinator_c_amd import build, layers, native
 
-SOURCES = ("expert_rows", "embed", "int8")
+SOURCES = ("expert_rows", "embed", "int8", "mx4")
 TYPES = {"f": "f32", "DF16b": "bf16", "DF16_": "f16"}
-ENTRIES = ("expert_rows", "expert_sum", "embed", "int8")
+ENTRIES = ("expert_rows", "expert_sum", "embed", "int8", "mx4")
 
 
 class Launch(NamedTuple):

@@ -21,7 +21,9 @@ WORDS = [("expert_rows_device", ROWS, ("offsets", "positions", "weights")),
          ("embed_order_device", ORDER, ("ids", "order")),
          ("embed_backward_device", EMBED_BACK, ("ids", "order", "dtable")),
          ("int8_product_device", PRODUCT, ("a_scales", "rows", "w_scales", "offsets", "bias",
-                                           "row_scale"))]
+                                           "row_scale")),
+         ("mx4_product_device", PRODUCT, ("a_scales", "rows", "w_scales", "offsets", "bias",
+                                          "row_scale"))]
 
 
 @pytest.fixture(scope="module")

@@ -749,7 +749,7 @@ extern "C" int tb_hip_mx4_product_device(const void *a_codes, const void *a_scal
         (!rows && m != a_rows) ||
         !known_act(act) || !known_type(dtype) || !multiple_of(a_codes, 16) ||
         !multiple_of(w_codes, 16) || !multiple_of(a_scales, 4) || !multiple_of(w_scales, 4) ||
-        !multiple_of(out, type_size(dtype)))
+        !words_ok(rows, offsets, bias, row_scale) || !multiple_of(out, type_size(dtype)))
         return 0;
     ProductArgs a = {};
     a.a_codes = static_cast<const unsigned char *>(a_codes);
